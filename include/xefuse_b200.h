@@ -60,7 +60,8 @@ typedef enum xf_dtype {
   XF_DT_BF16 = 0,
   XF_DT_S8 = 1,
   XF_DT_F32 = 2,
-  XF_DT_S32 = 3
+  XF_DT_S32 = 3,
+  XF_DT_E4M3 = 4  /* 8-bit floating point, largest value 448: block-scaled operands and outputs only */
 } xf_dtype;
 
 /* Unary activation applied after the affine steps
@@ -361,6 +362,34 @@ XF_API xf_status xf_ve_dequant_act_mul(void* out, const int32_t* acc, const floa
 XF_API xf_status xf_ve_dequant_rotary(void* out, const int32_t* acc, const float* scale_token,
                                       const float* scale_channel, const float* cos_sin, int M, int N,
                                       int L, void* stream);
+
+/*
+ * Row passes with an 8-bit output: the producers of 8-bit operands for the int8 GEMM (one scale per
+ * row) and the block-scaled products (one scale per row and block of 128 columns).  No counterpart in
+ * the reference, whose quantising pass takes neither residual nor weight and writes int8 only.
+ *
+ * out_dtype XF_DT_S8: code = round(v / scale), ties away from zero, scale = max|v| / 127 over the row,
+ * stored at scale[m * scale_row_stride].  XF_DT_E4M3: code = e4m3(v / scale), scale = max|v| / 448 over
+ * each block of 128 columns (the last one may be shorter), stored at
+ * scale[m * scale_row_stride + b * scale_blk_stride].  Maxima are floored at 2^-100 times the row's
+ * rstd, so zeros get zero codes and a finite scale; a NaN or an infinity makes the scale of its block
+ * NaN or infinite.  Pitches in elements, any value from the row's width up and any alignment; 16-byte
+ * aligned rows are faster.  N (d) up to 2^20.  M == 0 is an empty call.  All asynchronous on
+ * `stream`, of the current device; no workspace.
+ */
+/* v = RMSNorm(h) * weight with h = input, or, where residual is given, h = bf16(input + residual), which
+ * is written to residual_out (may be residual itself: the stream updated in place).  The mean square is
+ * taken over the rounded h.  weight bf16 [N] or NULL (ones). */
+XF_API xf_status xf_rms_norm_quantize(void* out, int out_dtype, int64_t ld_out, float* scale,
+                                      int64_t scale_row_stride, int64_t scale_blk_stride,
+                                      const void* input, int64_t ld_in, const void* residual,
+                                      int64_t ld_res, void* residual_out, int64_t ld_res_out,
+                                      const void* weight, int M, int N, float eps, void* stream);
+/* v[m,i] = act(input[m,i]) * input[m,d+i]; input bf16 [M,2d]; gelu=0 SiLU, 1 erf-GeLU. */
+XF_API xf_status xf_act_mul_quantize(void* out, int out_dtype, int64_t ld_out, float* scale,
+                                     int64_t scale_row_stride, int64_t scale_blk_stride,
+                                     const void* input, int64_t ld_in, int d, int M, int gelu,
+                                     void* stream);
 
 /*
  * Harness utilities behind the front end's cutlass/util shims (not on the fused path): the

@@ -1,0 +1,257 @@
+"""Row passes with an 8-bit output (xf_rms_norm_quantize, xf_act_mul_quantize) against 64-bit formulas.
+
+Tolerances, counted before the first run (u = 2^-24, the rounding of one fp32 operation):
+ * norm codes: t = h * w is exact, L / a and its product with t round once each, so the value that is rounded
+   to a code is within 2^-22 of the exact one; int8 codes near a tie are decided exactly, so they are equal.
+ * norm scales: a sum of n non-negative terms per thread and ten levels of tree add at most (n + 10) u to the
+   mean, half of it to rstd; division, root, product and division add 5 u.
+ * gate: __expf(x) is within 2 + 1.173 |x| ulp (2 u each), which a sigmoid passes on at most once;
+   the sum, the division (2 ulp) and the product with `up` add 8 u.  erf in gelu is within 1.5e-7 of 1 + erf.
+"""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+FLOOR = 2.0 ** -100
+E4M3 = torch.float8_e4m3fn
+
+
+def nearest_e4m3(v):
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -6))) - 3)
+    return (torch.round(v / step) * step).clamp(-448.0, 448.0)
+
+
+def nearest_s8(v):
+    return torch.sign(v) * torch.floor(v.abs() + 0.5)
+
+
+def block_max(t, s8):
+    """Largest magnitude of each row (s8) or block of 128 columns, floored, and the same for every element."""
+    M, N = t.shape
+    if s8:
+        a = t.abs().amax(1).clamp_min(FLOOR)
+        return a, a[:, None].expand(M, N)
+    p = torch.nn.functional.pad(t, (0, -N % 128)).view(M, -1, 128).abs().amax(2).clamp_min(FLOOR)
+    return p, p.repeat_interleave(128, 1)[:, :N]
+
+
+def padded(M, N, extra, dtype, gen=None, scale=1.0):
+    """[M, N] with `extra` columns of something else behind each row."""
+    t = torch.randn(M, N + extra, device="cuda", generator=gen).mul_(scale).to(dtype)
+    return t, t[:, :N]
+
+
+def out_tensors(M, N, s8, extra):
+    whole = torch.full((M, N + extra), 77, device="cuda", dtype=torch.int8)
+    q = (whole if s8 else whole.view(E4M3))[:, :N]
+    scale = torch.full((M,), -1.0, device="cuda") if s8 else torch.full((-(-N // 128), M), -1.0, device="cuda").t()
+    return whole, q, scale
+
+
+def check_norm(h, w, q, scale, s8, eps, threads_terms):
+    t = h.double() * (w.double() if w is not None else 1.0)
+    L = 127.0 if s8 else 448.0
+    a, wide = block_max(t, s8)
+    v = t * L / wide
+    if s8:
+        assert torch.equal(q.double(), nearest_s8(v))
+    else:
+        lo, hi = nearest_e4m3(v * (1 - 2.0 ** -22)), nearest_e4m3(v * (1 + 2.0 ** -22))
+        got = q.double()
+        assert bool(((got == lo) | (got == hi)).all())
+    rstd = 1.0 / torch.sqrt(h.double().square().mean(1) + eps)
+    want = a * (rstd if s8 else rstd[:, None]) / L
+    tol = ((threads_terms + 10) / 2 + 5) * U
+    assert bool(((scale.double() - want).abs() <= tol * want).all())
+
+
+NORM_SHAPES = [(1, 1), (1, 7), (3, 127), (2, 128), (5, 129), (4, 4096), (33, 5003), (2, 8200), (3, 20000), (2, 40001)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("s8", [False, True])
+@pytest.mark.parametrize("residual", [None, "apart", "in place"])
+@pytest.mark.parametrize("M,N", NORM_SHAPES)
+@pytest.mark.parametrize("extra", [0, 24, 5])
+def test_norm(capi, cuda, M, N, residual, s8, extra):
+    gen = torch.Generator(device="cuda").manual_seed(M * 100003 + N)
+    _, x = padded(M, N, extra, torch.bfloat16, gen)
+    w = torch.randn(N, device=cuda, generator=gen).to(torch.bfloat16) if extra != 5 else None
+    whole, q, scale = out_tensors(M, N, s8, extra)
+    res = hout = None
+    h = x
+    if residual:
+        rwhole, res = padded(M, N, extra, torch.bfloat16, gen, 3.0)
+        before = rwhole.clone()
+        h = (x.float() + res.float()).to(torch.bfloat16)
+        hout = torch.zeros(M, N, device=cuda, dtype=torch.bfloat16) if residual == "apart" else None
+    capi.rms_norm_quantize(q, scale, x, w, res, hout, 1e-5)
+    torch.cuda.synchronize()
+    terms = 8 * math.ceil(N / 8 / 1024)
+    check_norm(h, w, q, scale, s8, 1e-5, terms)
+    assert bool((whole[:, N:] == 77).all())
+    if residual:
+        assert torch.equal(hout if residual == "apart" else res, h)
+        want = before if residual == "apart" else torch.cat([h, before[:, N:]], 1)
+        assert torch.equal(rwhole, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("s8", [False, True])
+def test_norm_special_rows(capi, cuda, s8):
+    N = 384
+    x = torch.randn(6, N, device=cuda).to(torch.bfloat16)
+    x[0] = 0                                   # nothing but zeros
+    x[1, 128:256] = 0                          # one block of zeros
+    x[2, 200] = float("nan")
+    x[3, 5] = float("inf")
+    x[4] = 1e-38                               # far below the floor once squared
+    x[5] = 3e38                                # the sum of squares overflows: rstd is 0
+    _, q, scale = out_tensors(6, N, s8, 0)
+    capi.rms_norm_quantize(q, scale, x, None, eps=1e-6)
+    torch.cuda.synchronize()
+    v = q.double() * (scale.double()[:, None] if s8 else scale.double().repeat_interleave(128, 1))
+    assert bool((q[0].float() == 0).all()) and bool(torch.isfinite(scale[0]).all()) and bool((scale[0] > 0).all())
+    assert bool((q[1, 128:256].float() == 0).all())
+    check_norm(x[1:2], None, q[1:2], scale[1:2], s8, 1e-6, 8)
+    assert bool(torch.isnan(scale[2]).all())   # the row's mean is NaN
+    assert bool(torch.isnan(scale[3]).any())   # inf * rstd, rstd = 0
+    assert bool(torch.isfinite(v[4]).all()) and bool((v[4].abs() <= 1.001e-35).all())
+    assert bool((scale[5] == 0).all()) and bool(torch.isfinite(q[5].float()).all())
+
+
+def gate_tolerance(g, gelu):
+    if gelu:      # 1.5e-7 of a factor 1 + erf(z) that is at least 1 on the positive side; on the other
+        #           side P(t) exp(-z^2) with |error of P| <= 1.5e-7 / exp(-z^2) of P(0) = 1
+        z2 = g.abs().clamp_max(13.0).square() / 2
+        return torch.where(g >= 0, 3e-7 + 0 * g, 1.5e-7 * (1 + z2) * 8 + 1e-6)
+    return (2 * (2 + 1.173 * g.abs()) + 8) * U
+
+
+def check_act(x, d, q, scale, s8, gelu):
+    g, u = x[:, :d].double(), x[:, d:].double()
+    y = g * (torch.special.ndtr(g) if gelu else torch.sigmoid(g)) * u
+    L = 127.0 if s8 else 448.0
+    a, wide = block_max(y, s8)
+    # absolute slack of one value: its relative error, and for gelu the absolute error of 1 + erf
+    slack = (gate_tolerance(g, gelu) * y.abs()) + (1.5e-7 * (g * u).abs() if gelu else 0)
+    most, _ = block_max(slack, s8)
+    assert bool(((scale.double() * L - a).abs() <= most + 2 * U * a).all())
+    wide_scale = scale.double()[:, None].expand_as(y) if s8 else scale.double().repeat_interleave(128, 1)[:, :d]
+    got = q.double() * wide_scale
+    v = (y / wide_scale).abs()
+    half = 0.5 if s8 else torch.exp2(torch.floor(torch.log2(v.clamp_min(2.0 ** -6))) - 4)
+    # half a step at the value itself, and its slack seen from either side of a border
+    assert bool(((got - y).abs() <= half * wide_scale * (1 + 2.0 ** -20) + 2 * slack + 4 * U * y.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("s8", [False, True])
+@pytest.mark.parametrize("gelu", [False, True])
+@pytest.mark.parametrize("M,d", [(1, 1), (1, 8), (3, 127), (2, 128), (5, 129), (4, 4096), (17, 1003), (2, 14336), (3, 20001)])
+@pytest.mark.parametrize("extra", [0, 16, 3])
+def test_act(capi, cuda, M, d, gelu, s8, extra):
+    gen = torch.Generator(device="cuda").manual_seed(M * 100003 + d)
+    _, x = padded(M, 2 * d, extra, torch.bfloat16, gen, 2.0)
+    whole, q, scale = out_tensors(M, d, s8, extra)
+    capi.act_mul_quantize(q, scale, x, gelu)
+    torch.cuda.synchronize()
+    check_act(x, d, q, scale, s8, gelu)
+    assert bool((whole[:, d:] == 77).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("s8", [False, True])
+def test_act_special_values(capi, cuda, s8):
+    d = 256
+    x = torch.randn(4, 2 * d, device=cuda).to(torch.bfloat16)
+    x[0, d:] = 0                                 # up half of zeros
+    x[1, 3] = float("nan")
+    x[2, 7] = -100.0                             # exp(100) is infinite: the gate is -0
+    x[3, :d] = -200.0
+    _, q, scale = out_tensors(4, d, s8, 0)
+    capi.act_mul_quantize(q, scale, x)
+    torch.cuda.synchronize()
+    assert bool((q[0].float() == 0).all()) and bool(torch.isfinite(scale[0]).all())
+    assert bool(torch.isnan(scale[1].reshape(-1)[0]))
+    assert float(q[2, 7].float()) == 0.0 and bool(torch.isfinite(scale[2]).all())
+    assert bool((q[3].float() == 0).all())
+
+
+@pytest.mark.gpu
+def test_no_rows_and_other_streams(capi, cuda):
+    x = torch.randn(64, 512, device=cuda).to(torch.bfloat16)
+    _, q, scale = out_tensors(64, 512, False, 0)
+    capi.rms_norm_quantize(q[:0], scale[:0], x[:0])             # nothing to do, nothing written
+    capi.act_mul_quantize(q[:0, :256], scale[:0, :2], x[:0])
+    torch.cuda.synchronize()
+    assert bool((scale == -1).all())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        capi.rms_norm_quantize(q, scale, x)
+    side.synchronize()
+    want_q, want_s = q.clone(), scale.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        capi.rms_norm_quantize(q, scale, x)
+    for k in (1.0, 2.0):
+        q.view(torch.int8).zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(q.view(torch.int8), want_q.view(torch.int8)) and torch.equal(scale, want_s)
+
+
+# ------------------------------------------------------------------ refusals: no GPU is touched
+def norm_args(**k):
+    a = dict(out=0x1000, dt=4, ldo=512, s=0x2000, sr=1, sb=8, i=0x3000, ldi=512, r=None, ldr=0, h=None, ldh=0, w=None, M=8,
+             N=512, eps=1e-6, st=None)
+    a.update(k)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(M=-1), 4), (dict(N=0), 4), (dict(dt=0), 2), (dict(out=None), 4), (dict(s=None), 4), (dict(i=None), 4),
+    (dict(ldi=511), 3), (dict(ldo=511), 3), (dict(sr=0), 3), (dict(sb=0), 3), (dict(N=(1 << 20) + 1), 5),
+    (dict(i=0x3001), 1), (dict(s=0x2002), 1), (dict(r=0x4000, ldr=512), 4), (dict(h=0x4000, ldh=512), 4),
+    (dict(r=0x4000, ldr=511, h=0x4000, ldh=512), 3), (dict(r=0x4001, ldr=512, h=0x4000, ldh=512), 1), (dict(w=0x5001), 1),
+])
+def test_norm_refusals(capi, change, status):
+    assert capi.lib().xf_rms_norm_quantize(*norm_args(**change)) == status
+    assert capi.lib().xf_last_error_string()
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(M=-1), 4), (dict(d=0), 4), (dict(dt=3), 2), (dict(out=None), 4), (dict(ldi=1023), 3), (dict(ldo=511), 3),
+    (dict(d=(1 << 20) + 1), 5), (dict(i=0x3001), 1),
+])
+def test_act_refusals(capi, change, status):
+    a = dict(out=0x1000, dt=4, ldo=512, s=0x2000, sr=1, sb=8, i=0x3000, ldi=1024, d=512, M=8, gelu=0, st=None)
+    a.update(change)
+    assert capi.lib().xf_act_mul_quantize(*a.values()) == status
+
+
+def test_empty_calls(capi):
+    assert capi.lib().xf_rms_norm_quantize(*norm_args(M=0, out=None, i=None, s=None)) == 0
+    assert capi.lib().xf_act_mul_quantize(None, 4, 512, None, 1, 8, None, 1024, 512, 0, 0, None) == 0
+
+
+def test_wrapper_refusals(capi, monkeypatch):
+    monkeypatch.setattr(capi, "_on_current_device", lambda *t: None)
+    x, s = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(4, 2)
+    q = torch.zeros(4, 256, dtype=E4M3)
+    for bad in (
+        lambda: capi.rms_norm_quantize(torch.zeros(4, 256), s, x),                  # output type
+        lambda: capi.rms_norm_quantize(q, torch.zeros(4, 1), x),                    # scales of another width
+        lambda: capi.rms_norm_quantize(q, s, x.float()),                            # input type
+        lambda: capi.rms_norm_quantize(q[:, ::2], s, x),                            # another width
+        lambda: capi.rms_norm_quantize(q.t().contiguous().t(), s, x),               # columns not contiguous
+        lambda: capi.rms_norm_quantize(q, s, x, x[0, :128]),                        # weight of another width
+        lambda: capi.rms_norm_quantize(q, s, x, residual=x[:2]),
+        lambda: capi.act_mul_quantize(q, s, x),                                     # input is [M, 2 d]
+    ):
+        with pytest.raises(capi.XfError):
+            bad()

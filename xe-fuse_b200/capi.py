@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libxefuse_b200.so")
 
 # enums (include/xefuse_b200.h)
-DT_BF16, DT_S8, DT_F32, DT_S32 = 0, 1, 2, 3
+DT_BF16, DT_S8, DT_F32, DT_S32, DT_E4M3 = 0, 1, 2, 3, 4
 UNARY = {"none": 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "relu": 4, "sigmoid": 5, "exp": 6}
 PAIR = {"none": 0, "swiglu": 1, "geglu": 2, "rope": 3, "swap": 4}
 OUT_FULL, OUT_COMPACT = 0, 1
@@ -85,6 +85,7 @@ EXPORTS = [
     "xf_row_sumsq_count", "xf_reduce_partials_rsqrt",
     "xf_ve_rms_norm", "xf_ve_fused_add_rms_norm", "xf_ve_act_and_mul", "xf_ve_rotary_embedding",
     "xf_ve_dequant_act_mul", "xf_ve_dequant_rotary",
+    "xf_rms_norm_quantize", "xf_act_mul_quantize",
     "xf_harness_fill_uniform", "xf_harness_ref_gemm", "xf_harness_compare",
 ]
 
@@ -137,6 +138,9 @@ def lib():
     L.xf_ve_rotary_embedding.argtypes = [vp, vp, vp, i32, i32, i32, i32, i32, vp]
     L.xf_ve_dequant_act_mul.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, vp]
     L.xf_ve_dequant_rotary.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, vp]
+    i64 = C.c_int64
+    L.xf_rms_norm_quantize.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, vp, i64, vp, i64, vp, i32, i32, f32, vp]
+    L.xf_act_mul_quantize.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, i32, i32, i32, vp]
     _lib = L
     return L
 
@@ -148,7 +152,8 @@ def check(status):
 
 def _torch_dtype_code(t):
     import torch
-    return {torch.bfloat16: DT_BF16, torch.int8: DT_S8, torch.float32: DT_F32, torch.int32: DT_S32}[t.dtype]
+    return {torch.bfloat16: DT_BF16, torch.int8: DT_S8, torch.float32: DT_F32, torch.int32: DT_S32,
+            torch.float8_e4m3fn: DT_E4M3}[t.dtype]
 
 
 def vec(t, batch_stride=0, null_default=1.0):
@@ -377,6 +382,76 @@ def ve_dequant_rotary(out, acc, scale_token, scale_channel, cos_sin):
     L_, M, N = _lmn(out)
     check(lib().xf_ve_dequant_rotary(out.data_ptr(), acc.data_ptr(), scale_token.data_ptr(),
                                      scale_channel.data_ptr(), cos_sin.data_ptr(), M, N, L_, _stream()))
+
+
+# ---- row passes with an 8-bit output --------------------------------------------------------------
+def _rows(t, what, M, N, dtype):
+    """Checks a [M, N] tensor with contiguous columns and returns (pointer, row pitch)."""
+    if t.dtype != dtype:
+        raise XfError(2, f"{what}: expected {dtype}, got {t.dtype}")
+    if tuple(t.shape) != (M, N) or (N > 1 and t.stride(1) != 1):
+        raise XfError(3, f"{what}: expected a [{M}, {N}] tensor with contiguous columns, got "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+    return t.data_ptr(), (t.stride(0) if M > 1 else max(t.stride(0), N))
+
+
+def _on_current_device(*tensors):
+    import torch
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != cur:
+            raise XfError(4, f"tensor on {t.device}, but cuda:{cur} is the current device")
+
+
+def _scales(scale, dtype_code, M, N):
+    """Pointer and strides of the scales of an 8-bit [M, N] output."""
+    import torch
+    shape = (M,) if dtype_code == DT_S8 else (M, -(-N // 128))
+    if scale.dtype != torch.float32 or tuple(scale.shape) != shape:
+        raise XfError(3, f"scale: expected float32 {shape}, got {scale.dtype} {tuple(scale.shape)}")
+    # a dimension of one has no meaningful stride
+    return (scale.data_ptr(), scale.stride(0) if M > 1 else 1,
+            scale.stride(1) if dtype_code == DT_E4M3 and N > 128 else 1)
+
+
+def _code_dtype(out):
+    import torch
+    if out.dtype not in (torch.int8, torch.float8_e4m3fn):
+        raise XfError(2, f"out: int8 or float8_e4m3fn, got {out.dtype}")
+    return DT_S8 if out.dtype == torch.int8 else DT_E4M3
+
+
+def rms_norm_quantize(out, scale, inp, weight=None, residual=None, residual_out=None, eps=1e-6):
+    """out, scale = 8-bit RMSNorm(h) * weight, h = inp or inp + residual (written to residual_out, or in
+    place when that is None).  out int8 with scale [M], or float8_e4m3fn with scale [M, ceil(N/128)] of any
+    strides (the block-scaled products read fastest with the rows side by side: torch.empty(blocks, M).t())."""
+    import torch
+    M, N = inp.shape
+    code = _code_dtype(out)
+    if residual is not None and residual_out is None:
+        residual_out = residual
+    _on_current_device(out, scale, inp, weight, residual, residual_out)
+    if weight is not None and (weight.dtype != torch.bfloat16 or tuple(weight.shape) != (N,) or not weight.is_contiguous()):
+        raise XfError(3, f"weight: expected contiguous bfloat16 [{N}], got {weight.dtype} {tuple(weight.shape)}")
+    ip, il = _rows(inp, "inp", M, N, torch.bfloat16)
+    op, ol = _rows(out, "out", M, N, out.dtype)
+    rp, rl = _rows(residual, "residual", M, N, torch.bfloat16) if residual is not None else (None, 0)
+    hp, hl = _rows(residual_out, "residual_out", M, N, torch.bfloat16) if residual is not None else (None, 0)
+    sp, sr, sb = _scales(scale, code, M, N)
+    check(lib().xf_rms_norm_quantize(op, code, ol, sp, sr, sb, ip, il, rp, rl, hp, hl,
+                                     weight.data_ptr() if weight is not None else None, M, N, eps, _stream()))
+
+
+def act_mul_quantize(out, scale, inp, gelu=False):
+    """out, scale = 8-bit act(inp[:, :d]) * inp[:, d:]; inp [M, 2d]; out and scale as in rms_norm_quantize."""
+    import torch
+    M, d = out.shape
+    code = _code_dtype(out)
+    _on_current_device(out, scale, inp)
+    ip, il = _rows(inp, "inp", M, 2 * d, torch.bfloat16)
+    op, ol = _rows(out, "out", M, d, out.dtype)
+    sp, sr, sb = _scales(scale, code, M, d)
+    check(lib().xf_act_mul_quantize(op, code, ol, sp, sr, sb, ip, il, d, M, 1 if gelu else 0, _stream()))
 
 
 def reduce_partials_rsqrt(partials, rstd, M, N, L=1, eps=1e-6):

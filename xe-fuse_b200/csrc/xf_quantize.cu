@@ -1,0 +1,469 @@
+// Row passes with an 8-bit output: RMSNorm (optionally after a residual addition) and SwiGLU / GeGLU,
+// written as int8 with one scale per row or as e4m3 with one scale per row and block of 128 columns.
+//
+// Mathematics.  With h the (summed) input row, w the norm weight and rstd = 1/sqrt(mean h^2 + eps), the
+// normalised value is t * rstd, t = h * w.  A row's common factor cancels between a value and the
+// largest value of its block, so the codes need the row's sum of squares not at all:
+//     a     = max(max |t|, 2^-100)  over the block (e4m3) or the row (int8)
+//     code  = round(t * L / a)      L = 448 (e4m3, ties to even), 127 (int8, ties away from zero)
+//     scale = a * rstd / L
+// t is exact: a product of two bf16 values has 16 significant bits.  The floor of 2^-100 gives a block
+// of zeros zero codes and keeps L / a finite.  Maxima are taken over the bit patterns without the
+// sign, so a NaN is the largest of all and reaches the scale of its block.
+//
+// Bound.  All kernels move each byte once and are bound by HBM: 7 bytes per element with a residual
+// (x, r in; h, code out), 5 per output element of the gated form.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/xefuse_b200.h"
+#include "xf_act.cuh"
+#include "xf_host_util.h"
+#include "xf_ptx.cuh"
+
+namespace xf {
+namespace quantize {
+
+static const int kBlock = 128;        // columns that share a scale
+static const int kChunk = 8;          // columns a thread handles at a time: 16 bytes of bf16
+static const float kFloor = 7.888609052210118e-31f;   // 2^-100
+
+struct Params {
+  const __nv_bfloat16* in;
+  long long ld_in;
+  const __nv_bfloat16* residual;      // null: none
+  __nv_bfloat16* residual_out;        // the sum, where there is a residual
+  long long ld_res, ld_res_out;
+  const __nv_bfloat16* weight;        // null: ones
+  uint8_t* out;
+  long long ld_out;
+  float* scale;
+  long long scale_row, scale_blk;     // strides of the scales
+  int M, N;
+  float eps;
+  int vec_in, vec_res, vec_out;       // 1: rows of that tensor start where 16-byte (out: 8-byte) accesses may
+  int vec_w;
+  int row_bytes;                      // int8: bytes of shared memory that hold a row, 0: read it again
+};
+
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Columns [c0, c0 + 8) of a bf16 row; columns from N on read as zero.
+__device__ __forceinline__ uint4 load_chunk(const __nv_bfloat16* row, int c0, int N, int vec) {
+  if (vec && c0 + kChunk <= N) return *reinterpret_cast<const uint4*>(row + c0);
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+  uint32_t w[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint32_t lo = c0 + 2 * t < N ? p[c0 + 2 * t] : 0;
+    const uint32_t hi = c0 + 2 * t + 1 < N ? p[c0 + 2 * t + 1] : 0;
+    w[t] = lo | (hi << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store_chunk(__nv_bfloat16* row, int c0, int N, int vec, const uint4& u) {
+  if (vec && c0 + kChunk <= N) {
+    *reinterpret_cast<uint4*>(row + c0) = u;
+    return;
+  }
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i)
+    if (c0 + i < N) reinterpret_cast<uint16_t*>(row)[c0 + i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+}
+__device__ __forceinline__ void store_codes(uint8_t* row, int c0, int N, int vec, uint32_t lo, uint32_t hi) {
+  if (vec && c0 + kChunk <= N) {
+    *reinterpret_cast<uint2*>(row + c0) = make_uint2(lo, hi);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i)
+    if (c0 + i < N) row[c0 + i] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+}
+
+__device__ __forceinline__ void unpack(const uint4& u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    v[2 * t] = bf_lo(w[t]);
+    v[2 * t + 1] = bf_hi(w[t]);
+  }
+}
+__device__ __forceinline__ uint32_t absmax_bits(const float (&v)[8]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  return a;
+}
+
+// Two values to e4m3, round to nearest even, values beyond 448 to 448, NaN kept.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void codes_e4m3(const float (&t)[8], float a, uint32_t& lo, uint32_t& hi) {
+  const float inv = __fdiv_rn(448.0f, a);
+  lo = e4m3x2(t[0] * inv, t[1] * inv) | (e4m3x2(t[2] * inv, t[3] * inv) << 16);
+  hi = e4m3x2(t[4] * inv, t[5] * inv) | (e4m3x2(t[6] * inv, t[7] * inv) << 16);
+}
+// round(t * 127 / a), ties away from zero, of the exact quotient: the fp32 product is off by less
+// than 2^-15 at 127, so only a value that close to a border between two codes is decided by the exact
+// comparison 254 |t| >= (2 j - 1) a (both sides have at most 32 significant bits).
+__device__ __forceinline__ int code_s8(float t, float a, float inv) {
+  const float v = fabsf(t) * inv + 0.5f;
+  const float j = rintf(v);
+  float k = floorf(v);
+  if (fabsf(v - j) < 6.2e-5f)
+    k = 254.0 * static_cast<double>(fabsf(t)) >= (2.0 * j - 1.0) * static_cast<double>(a) ? j : j - 1.0f;
+  const int q = static_cast<int>(fminf(k, 127.0f));
+  return t < 0.0f ? -q : q;
+}
+__device__ __forceinline__ void codes_s8(const float (&t)[8], float a, uint32_t& lo, uint32_t& hi) {
+  const float inv = __fdiv_rn(127.0f, a);
+  lo = hi = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    lo |= (static_cast<uint32_t>(code_s8(t[i], a, inv)) & 0xFFu) << (8 * i);
+    hi |= (static_cast<uint32_t>(code_s8(t[4 + i], a, inv)) & 0xFFu) << (8 * i);
+  }
+}
+
+// Largest value over the 16 lanes that hold one block of 128 columns.
+__device__ __forceinline__ uint32_t max16(uint32_t a) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+  return a;
+}
+__device__ __forceinline__ float floored(uint32_t bits) {
+  return __uint_as_float(max(bits, __float_as_uint(kFloor)));   // NaN bits are above every number's
+}
+
+// Sum and bitwise maximum over the block; `red` holds 2 x 32 words.
+__device__ __forceinline__ void block_sum_max(float& s, uint32_t& m, uint32_t* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  m = __reduce_max_sync(0xffffffffu, m);
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31, nw = blockDim.x >> 5;
+  if (l == 0) {
+    red[w] = __float_as_uint(s);
+    red[32 + w] = m;
+  }
+  __syncthreads();
+  s = l < nw ? __uint_as_float(red[l]) : 0.0f;
+  m = l < nw ? red[32 + l] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  m = __reduce_max_sync(0xffffffffu, m);
+}
+
+// ---------------------------------------------------------------------------- norm
+// One block per row.  e4m3: one pass; the codes of a 128-column block leave as soon as its 16 lanes
+// know their maximum, the maxima wait in shared memory for the row's sum.  int8: the summed row waits in
+// shared memory for the row's maximum.
+template <bool S8>
+__global__ void __launch_bounds__(1024) rms_norm_kernel(const Params p) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ uint32_t red[64];
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
+  const long long row = blockIdx.x;
+  const __nv_bfloat16* xr = p.in + row * p.ld_in;
+  const __nv_bfloat16* rr = p.residual ? p.residual + row * p.ld_res : nullptr;
+  __nv_bfloat16* hr = p.residual ? p.residual_out + row * p.ld_res_out : nullptr;
+  uint8_t* qr = p.out + row * p.ld_out;
+  const int nchunk = (p.N + kChunk - 1) / kChunk;
+  const int lane = threadIdx.x & 31;
+  float ss = 0.0f;
+  uint32_t most = 0;
+  for (int c = threadIdx.x; c - lane < nchunk; c += blockDim.x) {
+    const int c0 = c * kChunk;
+    uint4 u = load_chunk(xr, c0, p.N, p.vec_in);
+    if (rr) {
+      const uint4 r = load_chunk(rr, c0, p.N, p.vec_res);
+      float a[8], b[8];
+      unpack(u, a);
+      unpack(r, b);
+      u = make_uint4(pack2(a[0] + b[0], a[1] + b[1]), pack2(a[2] + b[2], a[3] + b[3]),
+                     pack2(a[4] + b[4], a[5] + b[5]), pack2(a[6] + b[6], a[7] + b[7]));
+      store_chunk(hr, c0, p.N, p.vec_res, u);
+    }
+    float t[8];
+    unpack(u, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(t[i], t[i], ss);
+    if (p.weight) {
+      float w[8];
+      unpack(load_chunk(p.weight, c0, p.N, p.vec_w), w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] *= w[i];
+    }
+    const uint32_t mine = absmax_bits(t);
+    if (S8) {
+      most = max(most, mine);
+      if (p.row_bytes && c < nchunk) reinterpret_cast<uint4*>(dyn)[c] = u;
+    } else {
+      const uint32_t a = max16(mine);
+      uint32_t lo, hi;
+      codes_e4m3(t, floored(a), lo, hi);
+      store_codes(qr, c0, p.N, p.vec_out, lo, hi);
+      if ((lane & 15) == 0 && c < nchunk) reinterpret_cast<uint32_t*>(dyn)[c >> 4] = a;
+    }
+  }
+  block_sum_max(ss, most, red);
+  const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(ss / static_cast<float>(p.N) + p.eps));
+  if (!S8) {
+    const int nblk = (p.N + kBlock - 1) / kBlock;
+    for (int b = threadIdx.x; b < nblk; b += blockDim.x)
+      p.scale[row * p.scale_row + b * p.scale_blk] =
+          __fdiv_rn(floored(reinterpret_cast<const uint32_t*>(dyn)[b]) * rstd, 448.0f);
+    return;
+  }
+  const float a = floored(most);
+  if (threadIdx.x == 0) p.scale[row * p.scale_row] = __fdiv_rn(a * rstd, 127.0f);
+  const __nv_bfloat16* again = rr ? hr : xr;
+  for (int c = threadIdx.x; c < nchunk; c += blockDim.x) {
+    const int c0 = c * kChunk;
+    // a thread reads back what it wrote itself
+    const uint4 u = p.row_bytes ? reinterpret_cast<const uint4*>(dyn)[c]
+                                : load_chunk(again, c0, p.N, rr ? p.vec_res : p.vec_in);
+    float t[8];
+    unpack(u, t);
+    if (p.weight) {
+      float w[8];
+      unpack(load_chunk(p.weight, c0, p.N, p.vec_w), w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] *= w[i];
+    }
+    uint32_t lo, hi;
+    codes_s8(t, a, lo, hi);
+    store_codes(qr, c0, p.N, p.vec_out, lo, hi);
+  }
+}
+
+// ---------------------------------------------------------------------------- gate
+template <bool GELU>
+__device__ __forceinline__ void gated(const uint4& g, const uint4& u, float (&y)[8]) {
+  float a[8], b[8];
+  unpack(g, a);
+  unpack(u, b);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (GELU ? gelu_f(a[i]) : silu_f(a[i])) * b[i];
+}
+
+// e4m3: 16 lanes per block of 128 columns; nothing is shared beyond them.
+template <bool GELU>
+__global__ void __launch_bounds__(256) act_mul_e4m3_kernel(const Params p, uint32_t nblk, unsigned long long total) {
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
+  const unsigned long long b0 = (static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x) >> 4;
+  const bool live = b0 < total;                     // 16 lanes agree; the others of the warp take part in its shuffles
+  const unsigned long long b = live ? b0 : 0;
+  const long long row = static_cast<long long>(b / nblk);
+  const int blk = static_cast<int>(b - row * nblk);
+  const int c0 = blk * kBlock + (threadIdx.x & 15) * kChunk;
+  const __nv_bfloat16* xr = p.in + row * p.ld_in;
+  float y[8];
+  gated<GELU>(load_chunk(xr, c0, p.N, p.vec_in), load_chunk(xr + p.N, c0, p.N, p.vec_res), y);
+  const float a = floored(max16(absmax_bits(y)));
+  if (!live) return;
+  uint32_t lo, hi;
+  codes_e4m3(y, a, lo, hi);
+  store_codes(p.out + row * p.ld_out, c0, p.N, p.vec_out, lo, hi);
+  if ((threadIdx.x & 15) == 0) p.scale[row * p.scale_row + blk * p.scale_blk] = __fdiv_rn(a, 448.0f);
+}
+
+// int8: one block per row; the products wait in shared memory for the row's maximum, or are formed again
+// in a row too long for it.
+template <bool GELU>
+__global__ void __launch_bounds__(1024) act_mul_s8_kernel(const Params p) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ uint32_t red[64];
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
+  const long long row = blockIdx.x;
+  const __nv_bfloat16* xr = p.in + row * p.ld_in;
+  const int nchunk = (p.N + kChunk - 1) / kChunk;
+  float none = 0.0f;
+  uint32_t most = 0;
+  for (int c = threadIdx.x; c < nchunk; c += blockDim.x) {
+    float y[8];
+    gated<GELU>(load_chunk(xr, c * kChunk, p.N, p.vec_in), load_chunk(xr + p.N, c * kChunk, p.N, p.vec_res), y);
+    most = max(most, absmax_bits(y));
+    if (p.row_bytes) {
+      reinterpret_cast<float4*>(dyn)[c] = make_float4(y[0], y[1], y[2], y[3]);
+      reinterpret_cast<float4*>(dyn)[nchunk + c] = make_float4(y[4], y[5], y[6], y[7]);
+    }
+  }
+  block_sum_max(none, most, red);
+  const float a = floored(most);
+  if (threadIdx.x == 0) p.scale[row * p.scale_row] = __fdiv_rn(a, 127.0f);
+  for (int c = threadIdx.x; c < nchunk; c += blockDim.x) {
+    float y[8];
+    if (p.row_bytes) {
+      const float4 f = reinterpret_cast<const float4*>(dyn)[c], g = reinterpret_cast<const float4*>(dyn)[nchunk + c];
+      y[0] = f.x; y[1] = f.y; y[2] = f.z; y[3] = f.w;
+      y[4] = g.x; y[5] = g.y; y[6] = g.z; y[7] = g.w;
+    } else {
+      gated<GELU>(load_chunk(xr, c * kChunk, p.N, p.vec_in), load_chunk(xr + p.N, c * kChunk, p.N, p.vec_res), y);
+    }
+    uint32_t lo, hi;
+    codes_s8(y, a, lo, hi);
+    store_codes(p.out + row * p.ld_out, c * kChunk, p.N, p.vec_out, lo, hi);
+  }
+}
+
+// ---------------------------------------------------------------------------- host
+static int aligned(const void* p, long long pitch_bytes, int to) {
+  return (reinterpret_cast<uintptr_t>(p) % to) == 0 && pitch_bytes % to == 0;
+}
+
+static xf_status check(const char* what, const void* out, int out_dtype, int64_t ld_out, const float* scale,
+                       int64_t scale_row, int64_t scale_blk, const void* in, int64_t ld_in, int in_cols, int M, int N) {
+  if (M < 0 || N <= 0) {
+    set_error("%s: extents must be positive (M=%d N=%d)", what, M, N);
+    return XF_ERR_INVALID_PROBLEM;
+  }
+  if (out_dtype != XF_DT_S8 && out_dtype != XF_DT_E4M3) {
+    set_error("%s: the output is int8 or e4m3 (got dtype %d)", what, out_dtype);
+    return XF_ERR_INVALID_DATA_TYPE;
+  }
+  if (N > (1 << 20)) {
+    set_error("%s: rows of at most %d columns (got %d)", what, 1 << 20, N);
+    return XF_ERR_NOT_SUPPORTED;
+  }
+  if (M == 0) return XF_SUCCESS;
+  if (!out || !scale || !in) {
+    set_error("%s: null pointer", what);
+    return XF_ERR_INVALID_PROBLEM;
+  }
+  if (ld_in < in_cols || ld_out < N || scale_row < 1 || (out_dtype == XF_DT_E4M3 && N > kBlock && scale_blk < 1)) {
+    set_error("%s: pitches too small (ld_in=%lld ld_out=%lld scale strides %lld, %lld; N=%d)", what, (long long)ld_in,
+              (long long)ld_out, (long long)scale_row, (long long)scale_blk, N);
+    return XF_ERR_INVALID_LAYOUT;
+  }
+  if ((reinterpret_cast<uintptr_t>(in) & 1) || (reinterpret_cast<uintptr_t>(scale) & 3)) {
+    set_error("%s: pointers must be aligned to their element size", what);
+    return XF_ERR_MISALIGNED_OPERAND;
+  }
+  return XF_SUCCESS;
+}
+
+// Launches with programmatic stream serialization, like the products: the kernel waits for the previous
+// grid before its first global access.
+template <typename... Args>
+static xf_status launch(const char* what, void (*fn)(Args...), unsigned grid, unsigned threads, size_t smem, void* stream,
+                        Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, args...);
+  if (e != cudaSuccess) {
+    set_error("launch of %s failed: %s", what, cudaGetErrorString(e));
+    return XF_ERR_INTERNAL;
+  }
+  return XF_SUCCESS;
+}
+
+static unsigned row_threads(int N) {
+  const int chunks = (N + kChunk - 1) / kChunk;
+  const int t = (chunks + 31) / 32 * 32;
+  return t > 1024 ? 1024 : t;
+}
+
+static const int kRowBytes = 47 * 1024;   // rows up to this size wait in shared memory (48 KB need no opt-in)
+
+}  // namespace quantize
+}  // namespace xf
+
+extern "C" {
+
+xf_status xf_rms_norm_quantize(void* out, int out_dtype, int64_t ld_out, float* scale, int64_t scale_row_stride,
+                               int64_t scale_blk_stride, const void* input, int64_t ld_in, const void* residual,
+                               int64_t ld_res, void* residual_out, int64_t ld_res_out, const void* weight, int M,
+                               int N, float eps, void* stream) {
+  using namespace xf;
+  using namespace xf::quantize;
+  const char* what = "rms_norm_quantize";
+  xf_status s = quantize::check(what, out, out_dtype, ld_out, scale, scale_row_stride, scale_blk_stride, input, ld_in, N, M, N);
+  if (s != XF_SUCCESS || M == 0) return s;
+  if (!residual != !residual_out) {
+    set_error("%s: residual and residual_out go together", what);
+    return XF_ERR_INVALID_PROBLEM;
+  }
+  if (residual && (ld_res < N || ld_res_out < N)) {
+    set_error("%s: residual pitches %lld, %lld smaller than N=%d", what, (long long)ld_res, (long long)ld_res_out, N);
+    return XF_ERR_INVALID_LAYOUT;
+  }
+  if ((reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(residual_out) |
+       reinterpret_cast<uintptr_t>(weight)) & 1) {
+    set_error("%s: pointers must be aligned to their element size", what);
+    return XF_ERR_MISALIGNED_OPERAND;
+  }
+  Params p = {};
+  p.in = static_cast<const __nv_bfloat16*>(input); p.ld_in = ld_in;
+  p.residual = static_cast<const __nv_bfloat16*>(residual); p.ld_res = ld_res;
+  p.residual_out = static_cast<__nv_bfloat16*>(residual_out); p.ld_res_out = ld_res_out;
+  p.weight = static_cast<const __nv_bfloat16*>(weight);
+  p.out = static_cast<uint8_t*>(out); p.ld_out = ld_out;
+  p.scale = scale; p.scale_row = scale_row_stride; p.scale_blk = scale_blk_stride;
+  p.M = M; p.N = N; p.eps = eps;
+  p.vec_in = aligned(input, ld_in * 2, 16);
+  p.vec_res = residual && aligned(residual, ld_res * 2, 16) && aligned(residual_out, ld_res_out * 2, 16);
+  p.vec_out = aligned(out, ld_out, 8);
+  p.vec_w = aligned(weight, 0, 16);
+  const int nchunk = (N + kChunk - 1) / kChunk;
+  if (out_dtype == XF_DT_E4M3)
+    return launch(what, rms_norm_kernel<false>, M, row_threads(N), (nchunk + 15) / 16 * sizeof(uint32_t), stream, p);
+  p.row_bytes = nchunk * 16 <= kRowBytes ? nchunk * 16 : 0;
+  return launch(what, rms_norm_kernel<true>, M, row_threads(N), p.row_bytes, stream, p);
+}
+
+xf_status xf_act_mul_quantize(void* out, int out_dtype, int64_t ld_out, float* scale, int64_t scale_row_stride,
+                              int64_t scale_blk_stride, const void* input, int64_t ld_in, int d, int M, int gelu,
+                              void* stream) {
+  using namespace xf;
+  using namespace xf::quantize;
+  const char* what = "act_mul_quantize";
+  const int in_cols = d > (1 << 20) ? d : 2 * d;
+  xf_status s = quantize::check(what, out, out_dtype, ld_out, scale, scale_row_stride, scale_blk_stride, input, ld_in, in_cols, M, d);
+  if (s != XF_SUCCESS || M == 0) return s;
+  Params p = {};
+  p.in = static_cast<const __nv_bfloat16*>(input); p.ld_in = ld_in;
+  p.out = static_cast<uint8_t*>(out); p.ld_out = ld_out;
+  p.scale = scale; p.scale_row = scale_row_stride; p.scale_blk = scale_blk_stride;
+  p.M = M; p.N = d;
+  p.vec_in = aligned(input, ld_in * 2, 16);
+  p.vec_res = aligned(p.in + d, ld_in * 2, 16);      // the second half of the row
+  p.vec_out = aligned(out, ld_out, 8);
+  if (out_dtype == XF_DT_E4M3) {
+    const uint32_t nblk = (d + kBlock - 1) / kBlock;
+    const unsigned long long total = static_cast<unsigned long long>(M) * nblk;
+    const unsigned long long grid = (total + 15) / 16;
+    if (grid > 0x7FFFFFFFull) {
+      set_error("%s: more than 2^31 thread blocks (M=%d d=%d)", what, M, d);
+      return XF_ERR_NOT_SUPPORTED;
+    }
+    return gelu ? launch(what, act_mul_e4m3_kernel<true>, static_cast<unsigned>(grid), 256, 0, stream, p, nblk, total)
+                : launch(what, act_mul_e4m3_kernel<false>, static_cast<unsigned>(grid), 256, 0, stream, p, nblk, total);
+  }
+  const int nchunk = (d + kChunk - 1) / kChunk;
+  p.row_bytes = nchunk * 32 <= kRowBytes ? nchunk * 32 : 0;
+  return gelu ? launch(what, act_mul_s8_kernel<true>, M, row_threads(d), p.row_bytes, stream, p)
+              : launch(what, act_mul_s8_kernel<false>, M, row_threads(d), p.row_bytes, stream, p);
+}
+
+}  // extern "C"

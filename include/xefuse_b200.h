@@ -392,6 +392,72 @@ XF_API xf_status xf_act_mul_quantize(void* out, int out_dtype, int64_t ld_out, f
                                      void* stream);
 
 /*
+ * Products of ragged row groups, each with its own weight (the experts of a mixture, rows sorted by
+ * expert), in bf16 or block-scaled e4m3; with one group, the plain block-scaled e4m3 product.
+ *
+ *   D[m,:] = pair(A[m,:] * B[g])     group_offsets[g] <= m < group_offsets[g + 1]
+ *
+ * fp32 sums, rounded once to dtype_d.  e4m3 operands carry an fp32 scale for each block of 128 elements
+ * of a row of A (xf_rms_norm_quantize and xf_act_mul_quantize write them) and for each 128 x 128 block of
+ * B (the last blocks of K and N may be shorter):
+ *   A[m,k] stands for A[m,k] * scale_a[m * scale_a_row_stride + (k / 128) * scale_a_blk_stride]
+ *   B[k,n] of group g for B[k,n] * scale_b[g * scale_b_group_stride + (k / 128) * scale_b_k_stride
+ *                                          + (n / 128) * scale_b_n_stride]
+ * scale_a is read fastest with a row stride of 1.
+ *
+ * group_offsets are num_groups + 1 device int32, read by the kernel at each launch: the routing may change
+ * between launches of one plan (and of one captured graph) as long as the rows fit M.  They must not
+ * decrease; a group may be empty; rows outside [offsets[0], offsets[num_groups]) are neither read for a
+ * result nor written.  Offsets that break this leave D unspecified, but are clamped to [0, M]: nothing
+ * outside A and D is touched.  The reference's counterpart is the batched MoE expert kernel, one fixed
+ * row count for all experts (include/xe-fuse/kernels/gemm_moe_expert.hpp).
+ */
+typedef enum xf_b_layout {
+  XF_B_KN = 0,   /* B [G][K][N], N contiguous */
+  XF_B_NK = 1    /* B [G][N][K], K contiguous */
+} xf_b_layout;
+
+typedef struct xf_grouped_gemm_desc {
+  int32_t dtype_ab;              /* XF_DT_BF16 or XF_DT_E4M3 */
+  int32_t dtype_d;               /* XF_DT_BF16 or XF_DT_F32 */
+  int32_t M, N, K;               /* M: rows of A and D, all groups together; 0 is an empty problem */
+  int32_t num_groups;            /* 1..1024 */
+  const int32_t* group_offsets;  /* device [num_groups + 1]; NULL with one group: all M rows */
+  const void* A; int64_t lda;                    /* [M][K], K contiguous */
+  const void* B; int64_t ldb; int64_t batch_b;   /* batch_b 0: all groups share one weight */
+  int32_t b_layout;              /* xf_b_layout */
+  int32_t pair;                  /* XF_PAIR_NONE; XF_PAIR_SWIGLU / XF_PAIR_GEGLU: D is [M][N/2], one value
+                                    act(v[2j]) * v[2j+1] per pair of columns */
+  const float* scale_a; int64_t scale_a_row_stride, scale_a_blk_stride;          /* e4m3 only */
+  const float* scale_b; int64_t scale_b_k_stride, scale_b_n_stride, scale_b_group_stride;
+  void* D; int64_t ldd;          /* any alignment; 16-byte aligned rows are faster */
+  int32_t flags;                 /* XF_FLAG_FORCE_1CTA, _FORCE_2CTA, _NO_SPLIT, _NO_PDL, _SHORT_WAITS */
+  int32_t pad_;
+  uint64_t workspace_bytes;      /* size of the workspace handed to xf_grouped_gemm_plan_create */
+} xf_grouped_gemm_desc;
+
+typedef struct xf_grouped_plan xf_grouped_plan;
+
+/* Checks a problem without touching the GPU. */
+XF_API xf_status xf_grouped_gemm_can_implement(const xf_grouped_gemm_desc* desc);
+/* Bytes of device workspace the plan can use on the CURRENT device: status word, and the partial sums of
+ * tiles whose K range several CTAs share.  With less (desc.workspace_bytes) the plan runs whole tiles;
+ * with none a bounded wait that gives up is not reported. */
+XF_API xf_status xf_grouped_gemm_workspace_size(const xf_grouped_gemm_desc* desc, size_t* bytes);
+/* Copies the descriptor, picks a kernel, encodes tensor maps and clears the workspace's flags on `stream`:
+ * the first run must be ordered behind that.  The workspace belongs to one plan: launches of a plan (and of
+ * graphs that captured it) must not overlap one another, launches of plans with workspaces of their own
+ * may. */
+XF_API xf_status xf_grouped_gemm_plan_create(const xf_grouped_gemm_desc* desc, void* workspace,
+                                             void* stream, xf_grouped_plan** plan);
+/* Enqueues one launch on `stream` of the plan's device, which must be current. */
+XF_API xf_status xf_grouped_gemm_run(xf_grouped_plan* plan, void* stream);
+/* As xf_gemm_plan_device_status. */
+XF_API xf_status xf_grouped_gemm_plan_device_status(xf_grouped_plan* plan, int32_t* device_code);
+XF_API const char* xf_grouped_gemm_plan_kernel_name(const xf_grouped_plan* plan);
+XF_API xf_status xf_grouped_plan_destroy(xf_grouped_plan* plan);
+
+/*
  * Harness utilities behind the front end's cutlass/util shims (not on the fused path): the
  * seeded fill the harness mains call initialize_block, the naive device GEMM they use to rebuild
  * the expected accumulator (cutlass::reference::device::GemmComplex in tests/test_k1.cpp:113-117)

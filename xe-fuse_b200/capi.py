@@ -73,6 +73,23 @@ class XfGemmDesc(C.Structure):
                 ("D_peer", C.c_void_p * 7), ("workspace_bytes", C.c_uint64)]
 
 
+B_KN, B_NK = 0, 1
+
+
+class XfGroupedGemmDesc(C.Structure):
+    _fields_ = [("dtype_ab", C.c_int32), ("dtype_d", C.c_int32),
+                ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("num_groups", C.c_int32),
+                ("group_offsets", C.c_void_p),
+                ("A", C.c_void_p), ("lda", C.c_int64),
+                ("B", C.c_void_p), ("ldb", C.c_int64), ("batch_b", C.c_int64),
+                ("b_layout", C.c_int32), ("pair", C.c_int32),
+                ("scale_a", C.c_void_p), ("scale_a_row_stride", C.c_int64), ("scale_a_blk_stride", C.c_int64),
+                ("scale_b", C.c_void_p), ("scale_b_k_stride", C.c_int64), ("scale_b_n_stride", C.c_int64),
+                ("scale_b_group_stride", C.c_int64),
+                ("D", C.c_void_p), ("ldd", C.c_int64),
+                ("flags", C.c_int32), ("pad_", C.c_int32), ("workspace_bytes", C.c_uint64)]
+
+
 # Every symbol include/xefuse_b200.h declares (checked by the CPU test-suite).
 EXPORTS = [
     "xf_gemm_can_implement", "xf_gemm_workspace_size", "xf_gemm_plan_create", "xf_gemm_run",
@@ -86,6 +103,9 @@ EXPORTS = [
     "xf_ve_rms_norm", "xf_ve_fused_add_rms_norm", "xf_ve_act_and_mul", "xf_ve_rotary_embedding",
     "xf_ve_dequant_act_mul", "xf_ve_dequant_rotary",
     "xf_rms_norm_quantize", "xf_act_mul_quantize",
+    "xf_grouped_gemm_can_implement", "xf_grouped_gemm_workspace_size", "xf_grouped_gemm_plan_create",
+    "xf_grouped_gemm_run", "xf_grouped_gemm_plan_device_status", "xf_grouped_gemm_plan_kernel_name",
+    "xf_grouped_plan_destroy",
     "xf_harness_fill_uniform", "xf_harness_ref_gemm", "xf_harness_compare",
 ]
 
@@ -141,6 +161,14 @@ def lib():
     i64 = C.c_int64
     L.xf_rms_norm_quantize.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, vp, i64, vp, i64, vp, i32, i32, f32, vp]
     L.xf_act_mul_quantize.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, i32, i32, i32, vp]
+    L.xf_grouped_gemm_can_implement.argtypes = [C.POINTER(XfGroupedGemmDesc)]
+    L.xf_grouped_gemm_workspace_size.argtypes = [C.POINTER(XfGroupedGemmDesc), C.POINTER(C.c_size_t)]
+    L.xf_grouped_gemm_plan_create.argtypes = [C.POINTER(XfGroupedGemmDesc), vp, vp, C.POINTER(vp)]
+    L.xf_grouped_gemm_run.argtypes = [vp, vp]
+    L.xf_grouped_gemm_plan_device_status.argtypes = [vp, C.POINTER(C.c_int32)]
+    L.xf_grouped_gemm_plan_kernel_name.argtypes = [vp]
+    L.xf_grouped_gemm_plan_kernel_name.restype = C.c_char_p
+    L.xf_grouped_plan_destroy.argtypes = [vp]
     _lib = L
     return L
 
@@ -256,6 +284,90 @@ class GemmPlan:
             self.close()
         except Exception:
             pass
+
+
+class GroupedGemmPlan:
+    """D[m] = pair(A[m] @ B[g]) for the rows m of each group g; owns an xf_grouped_plan and its tensors.
+
+    A [M, K] and B in bfloat16, or in float8_e4m3fn with scale_a [M, ceil(K/128)] and scale_b; D [M, N]
+    ([M, N/2] with a pair op) in bfloat16 or float32.  B is [K, N], or [N, K] with b_nk; scale_b has one value
+    for each 128 x 128 block in B's order of dimensions.  With offsets (int32 [G + 1] on the GPU, read at each
+    run) B and scale_b have a leading dimension of G groups, or none: one weight shared by all."""
+
+    def __init__(self, A, B, D, *, offsets=None, scale_a=None, scale_b=None, b_nk=False, pair="none", flags=0):
+        import torch
+        L_ = lib()
+        self.handle = C.c_void_p()
+        self._keep = [A, B, D, offsets, scale_a, scale_b]
+        _on_current_device(*self._keep)
+        if B.dtype != A.dtype:
+            raise XfError(2, f"A and B must have one type, got {A.dtype} and {B.dtype}")
+        M, K = A.shape
+        N = B.shape[-2] if b_nk else B.shape[-1]
+        G = offsets.shape[0] - 1 if offsets is not None else 1
+        lead = () if B.dim() == 2 else (G,)
+        _rows(A, "A", M, K, A.dtype)
+        _rows(D, "D", M, N if pair == "none" else N // 2, D.dtype)
+        if tuple(B.shape) != lead + ((N, K) if b_nk else (K, N)) or (B.shape[-1] > 1 and B.stride(-1) != 1):
+            raise XfError(3, f"B: {tuple(B.shape)} with strides {B.stride()} does not fit A {tuple(A.shape)} and {G} groups")
+        if offsets is not None and (offsets.dtype != torch.int32 or offsets.dim() != 1 or not offsets.is_contiguous()):
+            raise XfError(2, "offsets: contiguous int32 vector expected")
+        d = XfGroupedGemmDesc()
+        d.dtype_ab, d.dtype_d = _torch_dtype_code(A), _torch_dtype_code(D)
+        d.M, d.N, d.K, d.num_groups = M, N, K, G
+        d.group_offsets = offsets.data_ptr() if offsets is not None else None
+        d.A, d.lda = A.data_ptr(), _pitch(A)
+        d.B, d.ldb, d.batch_b = B.data_ptr(), _pitch(B), (B.stride(0) if lead and G > 1 else 0)
+        d.b_layout = B_NK if b_nk else B_KN
+        d.pair = PAIR[pair]
+        d.D, d.ldd = D.data_ptr(), _pitch(D)
+        d.flags = flags
+        if A.dtype == torch.float8_e4m3fn and (scale_a is None or scale_b is None):
+            raise XfError(4, "float8_e4m3fn operands need scale_a and scale_b")
+        kb, nb = -(-K // 128), -(-N // 128)
+        if scale_a is not None:
+            if scale_a.dtype != torch.float32 or tuple(scale_a.shape) != (M, kb):
+                raise XfError(3, f"scale_a: expected float32 ({M}, {kb}), got {scale_a.dtype} {tuple(scale_a.shape)}")
+            d.scale_a, d.scale_a_row_stride, d.scale_a_blk_stride = scale_a.data_ptr(), scale_a.stride(0), scale_a.stride(1)
+        if scale_b is not None:
+            want = lead + ((nb, kb) if b_nk else (kb, nb))
+            if scale_b.dtype != torch.float32 or tuple(scale_b.shape) != want:
+                raise XfError(3, f"scale_b: expected float32 {want}, got {scale_b.dtype} {tuple(scale_b.shape)}")
+            d.scale_b = scale_b.data_ptr()
+            d.scale_b_k_stride, d.scale_b_n_stride = scale_b.stride(-1 if b_nk else -2), scale_b.stride(-2 if b_nk else -1)
+            d.scale_b_group_stride = scale_b.stride(0) if lead else 0
+        self.desc = d
+        check(L_.xf_grouped_gemm_can_implement(C.byref(d)))
+        ws = C.c_size_t(0)
+        check(L_.xf_grouped_gemm_workspace_size(C.byref(d), C.byref(ws)))
+        self.workspace = torch.empty(int(ws.value), dtype=torch.uint8, device=A.device)
+        d.workspace_bytes = self.workspace.numel()
+        check(L_.xf_grouped_gemm_plan_create(C.byref(d), self.workspace.data_ptr(), _stream(), C.byref(self.handle)))
+        self.kernel_name = L_.xf_grouped_gemm_plan_kernel_name(self.handle).decode()
+
+    def run(self, stream=None):
+        check(lib().xf_grouped_gemm_run(self.handle, stream if stream is not None else _stream()))
+
+    def device_status(self):
+        code = C.c_int32(0)
+        check(lib().xf_grouped_gemm_plan_device_status(self.handle, C.byref(code)))
+        return code.value
+
+    def close(self):
+        if self.handle:
+            lib().xf_grouped_plan_destroy(self.handle)
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _pitch(t):
+    """Row pitch of a matrix (or stack of matrices) with contiguous columns; a single row's is of no use."""
+    return t.stride(-2) if t.shape[-2] > 1 else -(-t.shape[-1] // 16) * 16
 
 
 def cluster_capacity(dtype_code=DT_BF16):

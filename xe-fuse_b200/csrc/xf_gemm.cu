@@ -45,9 +45,9 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-static bool encode_3d(CUtensorMap* tm, CUtensorMapDataType dt, const void* base, uint64_t d0,
-                      uint64_t d1, uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes,
-                      uint32_t b0, uint32_t b1, CUtensorMapSwizzle sw) {
+bool encode_3d(CUtensorMap* tm, CUtensorMapDataType dt, const void* base, uint64_t d0,
+               uint64_t d1, uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes,
+               uint32_t b0, uint32_t b1, CUtensorMapSwizzle sw) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) {
     set_error("cuTensorMapEncodeTiled is not available from this driver");

@@ -72,6 +72,7 @@ struct Cfg {
   static constexpr int STAGES = 6;
   static constexpr int NBUF = 512 / BN;                 // accumulators in TMEM
   static constexpr int NC = BN / 2;                     // columns per epilogue warp
+  static constexpr bool SPLIT_REGS = NC == 128;
   static constexpr int STG_BYTES = 2048;                // staging per epilogue warp: 32 rows x 64 bytes
   static constexpr int BAR_BYTES = 256;
   static constexpr int TAB_BYTES = (kMaxGroups + 1 + 2 * kMaxGroups) * 4;   // first tile, {first row, rows} of a group
@@ -128,6 +129,26 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Two fp32 values in one 64-bit register pair.
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t x, uint64_t f) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(f));
+}
+// acc += r * f for the 32 words r of a TMEM slice, two columns per instruction; f holds the factor twice.
+__device__ __forceinline__ void scale_add(uint64_t* acc, const uint4 (&r)[8], uint64_t f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    fma2(acc[2 * j], pair_of(r[j].x, r[j].y), f);
+    fma2(acc[2 * j + 1], pair_of(r[j].z, r[j].w), f);
+  }
+}
+
 // Writes 64 bytes of each of 32 rows (w: this lane's row) to row-major global memory through the warp's
 // staging buffer, so that four neighbouring lanes write one row's 64 bytes.  Chunks of 16 bytes are
 // swizzled by the row: both directions are free of bank conflicts.  ES: bytes per element.
@@ -180,11 +201,10 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   int* first = reinterpret_cast<int*>(staging + 8 * C::STG_BYTES + C::BAR_BYTES);   // [G + 1] first tile of a group
   int* grow = first + kMaxGroups + 1;            // [G][2] first row, rows
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t rank = CTAS > 1 ? ptx::cluster_ctarank() : 0u;
   const int unit = CTAS > 1 ? static_cast<int>(ptx::cluster_id_x()) : blockIdx.x;
   const int units = CTAS > 1 ? static_cast<int>(ptx::num_clusters_x()) : gridDim.x;
-  const long long budget = p.wait_budget;
 
   if (warp == 0 && lane == 0) {
     ptx::prefetch_tmap(&p.tm_a);
@@ -243,20 +263,22 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
     ptx::cluster_wait();
   }
   ptx::tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  Schedule sched = {unit, units, first[p.G], p.num_kb};
+  const uint32_t tmem = ptx::uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
+  Schedule sched = {unit, units, ptx::uniform(first[p.G]), p.num_kb};
   Item it;
-  auto fail = [&](int code) {
-    if (p.status) atomicCAS(p.status, DEV_OK, code);
-  };
+  ptx::Waiter w = {p.status, p.wait_budget};
 
+  // 128 sums and two slices of 32 columns per thread do not fit the 168 registers that 384 threads can have
+  // each: the first four warps hand theirs over (72 + 2 x 216 = 3 x 168).
+  if constexpr (C::SPLIT_REGS) {
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  }
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      bool ok = true;
-      while (ok && sched.next(it)) {
+      while (sched.next(it)) {
         const Tile x = decode<C>(p, first, grow, it.tile);
         // rows of A that this CTA needs, and the bytes that both CTAs of a pair load
         uint32_t bytes = 0;
@@ -271,11 +293,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         const int col = x.n0 + static_cast<int>(rank) * C::BN_CTA;
         const int bg = p.b_grouped ? x.g : 0;
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
-          if (!ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, budget)) {
-            fail(DEV_TIMEOUT_PRODUCER_EMPTY);
-            ok = false;
-            break;
-          }
+          w.wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, DEV_TIMEOUT_PRODUCER_EMPTY);
           const uint32_t own = ptx::smem_u32(&full_bar[stage]);
           const uint32_t bar = CTAS == 2 ? ptx::mapa(own, 0) : own;
           if (rank == 0) ptx::mbar_arrive_expect_tx(own, bytes);
@@ -300,111 +318,163 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       // nobody waited for them (the leader's barriers count both CTAs' bytes; the pair leaves together).
       if (rank == 0) {
         for (int s = 0; s < STAGES; ++s)
-          ptx::mbar_wait(ptx::smem_u32(&full_bar[s]), s < stage ? phase : phase ^ 1u, budget);
+          w.wait(ptx::smem_u32(&full_bar[s]), s < stage ? phase : phase ^ 1u, DEV_TIMEOUT_MMA_FULL);
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && rank == 0) {
+    // The whole warp walks the loop and one elected lane issues: addresses and descriptors then stay in
+    // uniform registers (with one lane in the loop, an MMA took 110 clocks to issue).
+    if (rank == 0) {
       // D fp32, A and B bf16 (1) or e4m3 (0), A K-major, B N-major unless the weights are [N][K]
       constexpr uint32_t fmt = KIND == KIND_BF16 ? 1u : 0u;
       const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((p.b_nk ? 0u : 1u) << 16) |
                              (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(C::TM >> 4) << 24);
       const uint32_t b_lbo = p.b_nk ? 16u : static_cast<uint32_t>(C::GRP_BYTES);
       const uint64_t b_step = p.b_nk ? 2u : static_cast<uint64_t>(C::UK * 128) >> 4;   // per MMA, in 16 bytes
+      const uint32_t smem0 = ptx::smem_u32(smem), full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
+      const uint32_t tfull0 = ptx::smem_u32(tfull_bar), tempty0 = ptx::smem_u32(tempty_bar);
       int stage = 0, buf = 0;
       uint32_t phase = 0, tphase = 0;
-      bool ok = true;
-      while (ok && sched.next(it)) {
+      while (sched.next(it)) {
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           const bool fresh = KIND == KIND_E4M3 || kb == it.kb0;          // starts an accumulator
           const bool done = KIND == KIND_E4M3 || kb + 1 == it.kb1;       // and completes it
-          if (fresh) {
-            if (!ptx::mbar_wait_cluster(ptx::smem_u32(&tempty_bar[buf]), tphase ^ 1u, budget)) {
-              fail(DEV_TIMEOUT_MMA_TMEM_EMPTY);
-              ok = false;
-              break;
-            }
-          }
-          if (!ptx::mbar_wait(ptx::smem_u32(&full_bar[stage]), phase, budget)) {
-            fail(DEV_TIMEOUT_MMA_FULL);
-            ok = false;
-            break;
-          }
+          if (fresh) w.wait(tempty0 + buf * 8, tphase ^ 1u, DEV_TIMEOUT_MMA_TMEM_EMPTY);
+          w.wait(full0 + stage * 8, phase, DEV_TIMEOUT_MMA_FULL);
           ptx::tc_fence_after();
-          const uint32_t sa = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
+          const uint32_t sa = smem0 + stage * C::STAGE_BYTES;
           const uint64_t adesc = ptx::make_smem_desc_sw128(sa, 16, 1024);
           const uint64_t bdesc = ptx::make_smem_desc_sw128(sa + C::A_BYTES, b_lbo, 1024);
           const uint32_t d = tmem + static_cast<uint32_t>(buf * BN);
+          if (ptx::elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            ptx::umma<KIND, CTAS>(d, adesc + static_cast<uint64_t>(2 * k), bdesc + k * b_step, idesc,
-                                  (!fresh || k > 0) ? 1u : 0u);
-          const uint32_t eb = ptx::smem_u32(&empty_bar[stage]);
-          ptx::umma_commit<CTAS>(eb);
-          if constexpr (CTAS == 2) ptx::umma_commit<CTAS>(ptx::mapa(eb, 1));
-          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-          if (done) {
-            const uint32_t tb = ptx::smem_u32(&tfull_bar[buf]);
-            ptx::umma_commit<CTAS>(tb);
-            if constexpr (CTAS == 2) ptx::umma_commit<CTAS>(ptx::mapa(tb, 1));
-            if (++buf == NBUF) { buf = 0; tphase ^= 1u; }
+            for (int k = 0; k < 4; ++k)
+              ptx::umma<KIND, CTAS>(d, adesc + static_cast<uint64_t>(2 * k), bdesc + k * b_step, idesc,
+                                    (!fresh || k > 0) ? 1u : 0u);
+            if constexpr (CTAS == 2) {
+              if (done) ptx::umma_commit_pair(tfull0 + buf * 8);
+              ptx::umma_commit_pair(empty0 + stage * 8);
+            } else {
+              if (done) ptx::umma_commit<1>(tfull0 + buf * 8);
+              ptx::umma_commit<1>(empty0 + stage * 8);
+            }
           }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          if (done && ++buf == NBUF) { buf = 0; tphase ^= 1u; }
         }
       }
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ promotion and epilogue
+    if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int q = warp & 3, half = (warp - 4) >> 2;
     uint8_t* stg = staging + (warp - 4) * C::STG_BYTES;
     const uint32_t lead = CTAS == 2 ? ptx::mapa(ptx::smem_u32(&tempty_bar[0]), 0) : ptx::smem_u32(&tempty_bar[0]);
     const uint32_t t_base = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * NC);
     const int ncols = p.pair == PAIR_NONE ? p.N : p.N >> 1;
+    const uint32_t tfull0 = ptx::smem_u32(tfull_bar);
     int buf = 0;
     uint32_t tphase = 0;
-    bool ok = true;
-    while (ok && sched.next(it)) {
+    while (sched.next(it)) {
       const Tile x = decode<C>(p, first, grow, it.tile);
       const int roff = static_cast<int>(rank) * 128 + q * 32;      // of this warp inside the tile
       const int rows = x.rows - roff;                              // of the group, from this warp's first on
       const int col = x.n0 + half * NC;
       const bool live = rows > 0 && col < p.N;                     // the warp has outputs here
-      const float* sa = nullptr;
-      const float* sb = nullptr;
-      if (KIND == KIND_E4M3 && live) {
-        sa = p.sa + (static_cast<long long>(x.row0) + roff + min(lane, rows - 1)) * p.sa_row;
-        sb = p.sb + static_cast<long long>(x.g) * p.sb_group + static_cast<long long>(col >> 7) * p.sb_n;
+      uint64_t sum[NC / 2];                    // columns 2 i and 2 i + 1
+#pragma unroll
+      for (int i = 0; i < NC / 2; ++i) sum[i] = 0;
+      // The tile's accumulators one after another, in slices of 32 columns: while a slice is scaled and added,
+      // the next one is on its way out of TMEM, across the end of an accumulator too (its successor's
+      // barrier is tested one slice ahead).  A buffer is free once its last slice has been read.
+      const int last = KIND == KIND_E4M3 ? it.kb1 - 1 : it.kb0;
+      uint4 r[2][8];
+      auto open = [&](int b, uint32_t ph) {
+        w.wait(tfull0 + b * 8, ph, DEV_TIMEOUT_EPI_TMEM_FULL);
+        __syncwarp();
+        ptx::tc_fence_after();
+      };
+      auto take = [&](float factor, bool more) {
+        const uint64_t f = pair_of(__float_as_uint(factor), __float_as_uint(factor));
+        const uint32_t t0 = t_base + static_cast<uint32_t>(buf * BN);
+        const int nbuf = buf + 1 == NBUF ? 0 : buf + 1;
+        const uint32_t nphase = nbuf == 0 ? tphase ^ 1u : tphase;
+        bool ready = false;
+#pragma unroll
+        for (int c = 0; c < NC / 32; ++c) {
+          ptx::tmem_ld_wait_for(r[c & 1]);
+          if (c + 1 < NC / 32) {
+            ptx::tmem_ld_32x32_async(t0 + static_cast<uint32_t>((c + 1) * 32), r[(c + 1) & 1]);
+            if (c + 2 == NC / 32) ready = more && __all_sync(0xffffffffu, ptx::mbar_try_wait(tfull0 + nbuf * 8, nphase));
+          } else {
+            ptx::tc_fence_before();
+            if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead + static_cast<uint32_t>(buf * 8));
+            if (ready) {
+              ptx::tc_fence_after();
+              ptx::tmem_ld_32x32_async(t_base + static_cast<uint32_t>(nbuf * BN), r[0]);
+            }
+          }
+          scale_add(&sum[c * 16], r[c & 1], f);
+        }
+        if (more && !ready) {
+          open(nbuf, nphase);
+          ptx::tmem_ld_32x32_async(t_base + static_cast<uint32_t>(nbuf * BN), r[0]);
+        }
+        buf = nbuf;
+        tphase = nphase;
+      };
+      if (!live) {                                // nothing to add, but every accumulator is released by all
+        for (int kb = it.kb0; kb <= last; ++kb) {
+          open(buf, tphase);
+          ptx::tc_fence_before();
+          if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead + static_cast<uint32_t>(buf * 8));
+          if (++buf == NBUF) { buf = 0; tphase ^= 1u; }
+        }
+        continue;
+      }
+      if constexpr (KIND == KIND_BF16) {
+        open(buf, tphase);
+        ptx::tmem_ld_32x32_async(t_base + static_cast<uint32_t>(buf * BN), r[0]);
+        take(1.0f, false);
+      } else {
+        // Block scales are asked for two blocks ahead of their use.
+        const float* sa = p.sa + (static_cast<long long>(x.row0) + roff + min(lane, rows - 1)) * p.sa_row + it.kb0 * p.sa_blk;
+        const float* sb = p.sb + static_cast<long long>(x.g) * p.sb_group + static_cast<long long>(col >> 7) * p.sb_n +
+                          it.kb0 * p.sb_k;
+        float a0 = ptx::ld_early(sa), b0 = ptx::ld_early(sb), a1 = 0.0f, b1 = 0.0f;
+        if (it.kb0 < last) {
+          a1 = ptx::ld_early(sa + p.sa_blk);
+          b1 = ptx::ld_early(sb + p.sb_k);
+        }
+        open(buf, tphase);
+        ptx::tmem_ld_32x32_async(t_base + static_cast<uint32_t>(buf * BN), r[0]);
+#pragma unroll 1
+        for (int kb = it.kb0; kb <= last; kb += 2) {
+          sa += 2 * p.sa_blk;
+          sb += 2 * p.sb_k;
+          const float f0 = a0 * b0;
+          if (kb + 2 <= last) {
+            a0 = ptx::ld_early(sa);
+            b0 = ptx::ld_early(sb);
+          }
+          take(f0, kb < last);
+          if (kb == last) break;
+          const float f1 = a1 * b1;
+          if (kb + 3 <= last) {
+            a1 = ptx::ld_early(sa + p.sa_blk);
+            b1 = ptx::ld_early(sb + p.sb_k);
+          }
+          take(f1, kb + 1 < last);
+        }
       }
       float acc[NC];
 #pragma unroll
-      for (int i = 0; i < NC; ++i) acc[i] = 0.0f;
-      const int segs = KIND == KIND_E4M3 ? it.kb1 - it.kb0 : 1;
-      for (int s = 0; s < segs; ++s) {
-        float f = 1.0f;
-        if (KIND == KIND_E4M3 && live) f = sa[(it.kb0 + s) * p.sa_blk] * sb[(it.kb0 + s) * p.sb_k];
-        if (!ptx::mbar_wait(ptx::smem_u32(&tfull_bar[buf]), tphase, budget)) {
-          if (lane == 0) fail(DEV_TIMEOUT_EPI_TMEM_FULL);
-          ok = false;
-          break;
-        }
-        ptx::tc_fence_after();
-        if (live) {
-#pragma unroll
-          for (int c = 0; c < NC; c += 32) {
-            uint32_t r[32];
-            ptx::tmem_ld_32x32(t_base + static_cast<uint32_t>(buf * BN + c), r);
-            ptx::tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              acc[c + i] = KIND == KIND_E4M3 ? fmaf(__uint_as_float(r[i]), f, acc[c + i]) : __uint_as_float(r[i]);
-          }
-        }
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster(lead + static_cast<uint32_t>(buf * 8));
-        if (++buf == NBUF) { buf = 0; tphase ^= 1u; }
+      for (int i = 0; i < NC / 2; ++i) {
+        acc[2 * i] = lo_of(sum[i]);
+        acc[2 * i + 1] = hi_of(sum[i]);
       }
-      if (!ok || !live) continue;
       if (p.pair != PAIR_NONE) {
 #pragma unroll
         for (int i = 0; i < NC / 2; ++i)
@@ -461,6 +531,8 @@ struct Variant {
 };
 #define XF_GG(KIND, BN, CTAS, NAME) {KIND, BN, CTAS, Cfg<KIND, BN, CTAS>::SMEM_BYTES, grouped_gemm_kernel<KIND, BN, CTAS>, NAME}
 static const Variant g_variants[] = {
+    XF_GG(KIND_E4M3, 256, 2, "e4m3_256x256_cta2"),
+    XF_GG(KIND_BF16, 256, 2, "bf16_256x256_cta2"),
     XF_GG(KIND_E4M3, 128, 1, "e4m3_128x128_cta1"),
     XF_GG(KIND_BF16, 128, 1, "bf16_128x128_cta1"),
 };
@@ -578,8 +650,13 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
   }
   const int kind = d->dtype_ab == XF_DT_BF16 ? KIND_BF16 : KIND_E4M3;
   const Variant* v = nullptr;
+  // Pairs of CTAs on 256 x 256 tiles need half the operand bytes per multiplication of single CTAs on
+  // 128 x 128 tiles, which waste less on groups of few rows.
+  int ctas = d->M / d->num_groups > 128 ? 2 : 1;
+  if (d->flags & XF_FLAG_FORCE_1CTA) ctas = 1;
+  else if (d->flags & XF_FLAG_FORCE_2CTA) ctas = 2;
   for (const Variant& c : g_variants)
-    if (c.kind == kind) v = &c;
+    if (c.kind == kind && c.ctas == ctas) v = &c;
   const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(v->fn),
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, v->smem);
   if (e != cudaSuccess) {
@@ -588,7 +665,22 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
   }
   g->v = v;
   g->dev = dev;
-  g->units = sms / v->ctas;
+  g->units = sms;
+  if (v->ctas > 1) {   // pairs that can run at once: GPC boundaries may leave SMs without a partner
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms - sms % v->ctas, 1, 1);
+    cfg.blockDim = dim3(384, 1, 1);
+    cfg.dynamicSmemBytes = v->smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = v->ctas; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&g->units, reinterpret_cast<const void*>(v->fn), &cfg) != cudaSuccess || g->units < 1) {
+      cudaGetLastError();
+      g->units = sms / v->ctas;
+    }
+  }
   g->workspace_bytes = 256;
   return XF_SUCCESS;
 }

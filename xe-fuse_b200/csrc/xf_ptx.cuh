@@ -85,6 +85,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
                : "memory");
 }
+// The same arrival without memory ordering, for barriers that only say "my tcgen05 loads are complete":
+// the releasing form first waits for all of the thread's outstanding memory traffic.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+               : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
@@ -142,6 +148,31 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
     }
   }
   return true;
+}
+
+// A role's bounded waits.  One that runs out writes its code to the status word and lets the role go on
+// without waiting again for long: the launch is lost, but every role still walks its whole list and control
+// flow does not depend on a wait's outcome (a loop that a wait may leave keeps its counters, and with them
+// the operands of tensor-core instructions, out of uniform registers).
+struct Waiter {
+  int* status;
+  long long budget;
+  __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, int code) {
+    if (!mbar_wait(bar, parity, budget)) {
+      if (status) atomicCAS(status, 0, code);
+      budget = 0;
+    }
+  }
+};
+
+// A value that is the same in all lanes, known as such to the compiler.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// Read-only 4-byte load that the compiler may not move to where its value is used.
+__device__ __forceinline__ float ld_early(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
 }
 
 // 16-byte store into the shared memory of another CTA of the cluster (address from mapa).
@@ -383,6 +414,23 @@ __device__ __forceinline__ void umma_commit(uint32_t cluster_bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                      cluster_bar)
                  : "memory");
+}
+
+// The same for the barrier at this shared-memory offset in both CTAs of the pair (cluster ranks 0 and 1).
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+// True in one lane of a converged warp; the compiler knows that it is one, so that operands of the
+// instructions behind it may stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
 }
 
 // 64-bit shared-memory matrix descriptor, 128-byte swizzle, sm_100 version field set.

@@ -140,10 +140,10 @@ __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float(stat
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t x, uint64_t f) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(f));
 }
-// acc += r * f for the 32 words r of a TMEM slice, two columns per instruction; f holds the factor twice.
-__device__ __forceinline__ void scale_add(uint64_t* acc, const uint4 (&r)[8], uint64_t f) {
+// acc += r * f for the 16 words r of a TMEM slice, two columns per instruction; f holds the factor twice.
+__device__ __forceinline__ void scale_add(uint64_t* acc, const uint4 (&r)[4], uint64_t f) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     fma2(acc[2 * j], pair_of(r[j].x, r[j].y), f);
     fma2(acc[2 * j + 1], pair_of(r[j].z, r[j].w), f);
   }
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   Item it;
   ptx::Waiter w = {p.status, p.wait_budget};
 
-  // 128 sums and two slices of 32 columns per thread do not fit the 168 registers that 384 threads can have
+  // 128 sums and two slices of 16 columns per thread do not fit the 168 registers that 384 threads can have
   // each: the first four warps hand theirs over (72 + 2 x 216 = 3 x 168).
   if constexpr (C::SPLIT_REGS) {
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -340,13 +340,15 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           const bool fresh = KIND == KIND_E4M3 || kb == it.kb0;          // starts an accumulator
           const bool done = KIND == KIND_E4M3 || kb + 1 == it.kb1;       // and completes it
-          if (fresh) w.wait(tempty0 + buf * 8, tphase ^ 1u, DEV_TIMEOUT_MMA_TMEM_EMPTY);
           w.wait(full0 + stage * 8, phase, DEV_TIMEOUT_MMA_FULL);
-          ptx::tc_fence_after();
           const uint32_t sa = smem0 + stage * C::STAGE_BYTES;
           const uint64_t adesc = ptx::make_smem_desc_sw128(sa, 16, 1024);
           const uint64_t bdesc = ptx::make_smem_desc_sw128(sa + C::A_BYTES, b_lbo, 1024);
           const uint32_t d = tmem + static_cast<uint32_t>(buf * BN);
+          // last of all, the wait that the promotion warps answer: what follows it is on their round trip
+          if (fresh) w.wait(tempty0 + buf * 8, tphase ^ 1u, DEV_TIMEOUT_MMA_TMEM_EMPTY);
+          __syncwarp();
+          ptx::tc_fence_after();
           if (ptx::elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -386,44 +388,32 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       uint64_t sum[NC / 2];                    // columns 2 i and 2 i + 1
 #pragma unroll
       for (int i = 0; i < NC / 2; ++i) sum[i] = 0;
-      // The tile's accumulators one after another, in slices of 32 columns: while a slice is scaled and added,
-      // the next one is on its way out of TMEM, across the end of an accumulator too (its successor's
-      // barrier is tested one slice ahead).  A buffer is free once its last slice has been read.
+      // The tile's accumulators one after another, in slices of 16 columns: while a slice is scaled and added,
+      // the next one is on its way out of TMEM.  A buffer is free once its last slice has been read.
       const int last = KIND == KIND_E4M3 ? it.kb1 - 1 : it.kb0;
-      uint4 r[2][8];
+      uint4 r[2][4];
       auto open = [&](int b, uint32_t ph) {
         w.wait(tfull0 + b * 8, ph, DEV_TIMEOUT_EPI_TMEM_FULL);
         __syncwarp();
         ptx::tc_fence_after();
       };
-      auto take = [&](float factor, bool more) {
+      auto take = [&](float factor) {
+        open(buf, tphase);
         const uint64_t f = pair_of(__float_as_uint(factor), __float_as_uint(factor));
         const uint32_t t0 = t_base + static_cast<uint32_t>(buf * BN);
-        const int nbuf = buf + 1 == NBUF ? 0 : buf + 1;
-        const uint32_t nphase = nbuf == 0 ? tphase ^ 1u : tphase;
-        bool ready = false;
+        ptx::tmem_ld_32x16_async(t0, r[0]);
 #pragma unroll
-        for (int c = 0; c < NC / 32; ++c) {
+        for (int c = 0; c < NC / 16; ++c) {
           ptx::tmem_ld_wait_for(r[c & 1]);
-          if (c + 1 < NC / 32) {
-            ptx::tmem_ld_32x32_async(t0 + static_cast<uint32_t>((c + 1) * 32), r[(c + 1) & 1]);
-            if (c + 2 == NC / 32) ready = more && __all_sync(0xffffffffu, ptx::mbar_try_wait(tfull0 + nbuf * 8, nphase));
+          if (c + 1 < NC / 16) {
+            ptx::tmem_ld_32x16_async(t0 + static_cast<uint32_t>((c + 1) * 16), r[(c + 1) & 1]);
           } else {
             ptx::tc_fence_before();
             if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead + static_cast<uint32_t>(buf * 8));
-            if (ready) {
-              ptx::tc_fence_after();
-              ptx::tmem_ld_32x32_async(t_base + static_cast<uint32_t>(nbuf * BN), r[0]);
-            }
           }
-          scale_add(&sum[c * 16], r[c & 1], f);
+          scale_add(&sum[c * 8], r[c & 1], f);
         }
-        if (more && !ready) {
-          open(nbuf, nphase);
-          ptx::tmem_ld_32x32_async(t_base + static_cast<uint32_t>(nbuf * BN), r[0]);
-        }
-        buf = nbuf;
-        tphase = nphase;
+        if (++buf == NBUF) { buf = 0; tphase ^= 1u; }
       };
       if (!live) {                                // nothing to add, but every accumulator is released by all
         for (int kb = it.kb0; kb <= last; ++kb) {
@@ -435,9 +425,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         continue;
       }
       if constexpr (KIND == KIND_BF16) {
-        open(buf, tphase);
-        ptx::tmem_ld_32x32_async(t_base + static_cast<uint32_t>(buf * BN), r[0]);
-        take(1.0f, false);
+        take(1.0f);
       } else {
         // Block scales are asked for two blocks ahead of their use.
         const float* sa = p.sa + (static_cast<long long>(x.row0) + roff + min(lane, rows - 1)) * p.sa_row + it.kb0 * p.sa_blk;
@@ -448,8 +436,6 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
           a1 = ptx::ld_early(sa + p.sa_blk);
           b1 = ptx::ld_early(sb + p.sb_k);
         }
-        open(buf, tphase);
-        ptx::tmem_ld_32x32_async(t_base + static_cast<uint32_t>(buf * BN), r[0]);
 #pragma unroll 1
         for (int kb = it.kb0; kb <= last; kb += 2) {
           sa += 2 * p.sa_blk;
@@ -459,14 +445,14 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
             a0 = ptx::ld_early(sa);
             b0 = ptx::ld_early(sb);
           }
-          take(f0, kb < last);
+          take(f0);
           if (kb == last) break;
           const float f1 = a1 * b1;
           if (kb + 3 <= last) {
             a1 = ptx::ld_early(sa + p.sa_blk);
             b1 = ptx::ld_early(sb + p.sb_k);
           }
-          take(f1, kb + 1 < last);
+          take(f1);
         }
       }
       float acc[NC];

@@ -109,6 +109,21 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// The same question without waiting for the answer to change: try_wait may suspend the thread for a while.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Bounded wait.  `budget_cycles` is a clock64() budget (a few seconds); the clock is only read
 // every 256 failed polls so the common path costs nothing.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, long long budget_cycles) {
@@ -353,6 +368,26 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint4 (&a)[8]) {
                  "+r"(a[4].z), "+r"(a[4].w), "+r"(a[5].x), "+r"(a[5].y), "+r"(a[5].z), "+r"(a[5].w),
                  "+r"(a[6].x), "+r"(a[6].y), "+r"(a[6].z), "+r"(a[6].w), "+r"(a[7].x), "+r"(a[7].y),
                  "+r"(a[7].z), "+r"(a[7].w)
+               :
+               : "memory");
+}
+
+// 16 columns in four register groups, for loops that hold many other registers.
+__device__ __forceinline__ void tmem_ld_32x16_async(uint32_t taddr, uint4 (&a)[4]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(a[0].x), "=r"(a[0].y), "=r"(a[0].z), "=r"(a[0].w), "=r"(a[1].x), "=r"(a[1].y), "=r"(a[1].z),
+        "=r"(a[1].w), "=r"(a[2].x), "=r"(a[2].y), "=r"(a[2].z), "=r"(a[2].w), "=r"(a[3].x), "=r"(a[3].y),
+        "=r"(a[3].z), "=r"(a[3].w)
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait_for(uint4 (&a)[4]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(a[0].x), "+r"(a[0].y), "+r"(a[0].z), "+r"(a[0].w), "+r"(a[1].x), "+r"(a[1].y),
+                 "+r"(a[1].z), "+r"(a[1].w), "+r"(a[2].x), "+r"(a[2].y), "+r"(a[2].z), "+r"(a[2].w),
+                 "+r"(a[3].x), "+r"(a[3].y), "+r"(a[3].z), "+r"(a[3].w)
                :
                : "memory");
 }

@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libxefuse_b200.so")
 SOURCES = ["xf_gemm.cu", "xf_gemm_class_scale.cu", "xf_gemm_class_mat.cu", "xf_gemm_class_glu.cu",
            "xf_gemm_class_rope.cu", "xf_gemm_class_all.cu", "xf_standalone.cu", "xf_rowops.cu", "xf_quantize.cu",
-           "xf_grouped_gemm.cu", "xf_harness.cu"]
+           "xf_grouped_gemm.cu", "xf_grouped_gemm_bf16.cu", "xf_grouped_gemm_e4m3.cu", "xf_harness.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

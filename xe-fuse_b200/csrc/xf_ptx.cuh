@@ -168,14 +168,17 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
 // A role's bounded waits.  One that runs out writes its code to the status word and lets the role go on
 // without waiting again for long: the launch is lost, but every role still walks its whole list and control
 // flow does not depend on a wait's outcome (a loop that a wait may leave keeps its counters, and with them
-// the operands of tensor-core instructions, out of uniform registers).
+// the operands of tensor-core instructions, out of uniform registers).  P: kernel parameters with `status`
+// and `wait_budget`, which are read where they are needed and take no registers meanwhile.
+template <class P>
 struct Waiter {
-  int* status;
-  long long budget;
+  const P& p;
+  bool lost;
   __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, int code) {
-    if (!mbar_wait(bar, parity, budget)) {
-      if (status) atomicCAS(status, 0, code);
-      budget = 0;
+    if (mbar_try_wait(bar, parity)) return;
+    if (!mbar_wait(bar, parity, lost ? 0 : p.wait_budget)) {
+      if (p.status) atomicCAS(p.status, 0, code);
+      lost = true;
     }
   }
 };

@@ -110,7 +110,8 @@ struct Geometry {
   const Variant* v;
   KernelFn fn;
   int dev, units;
-  size_t workspace_bytes;
+  int split_kb;            // 0: whole tiles only
+  size_t partials_off, workspace_bytes;   // [0, 256) status, flags, partial sums
 };
 
 static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
@@ -162,7 +163,11 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
       g->units = sms / v->ctas;
     }
   }
-  g->workspace_bytes = 256;
+  g->split_kb = d->flags & XF_FLAG_NO_SPLIT ? 0 : v->ctas == 2 ? 8 : 6;
+  if ((d->K + 63) / 64 > (1 << 20)) g->split_kb = 0;   // block numbers of a whole wave stay within 32 bits
+  const size_t grid = static_cast<size_t>(g->units) * v->ctas;
+  g->partials_off = 256 + (grid * 8 * sizeof(int) + 255) / 256 * 256;
+  g->workspace_bytes = g->split_kb ? g->partials_off + grid * 128 * v->bn * sizeof(float) : 256;
   return XF_SUCCESS;
 }
 
@@ -275,6 +280,13 @@ xf_status xf_grouped_gemm_plan_create(const xf_grouped_gemm_desc* d, void* works
   if (workspace && d->workspace_bytes >= 256) {
     p.status = static_cast<int*>(workspace);
     plan->clear_bytes = 256;
+    if (g.split_kb && d->workspace_bytes >= g.workspace_bytes) {
+      p.split_kb = g.split_kb;
+      p.flags = reinterpret_cast<int*>(static_cast<char*>(workspace) + 256);
+      p.partials = reinterpret_cast<float4*>(static_cast<char*>(workspace) + g.partials_off);
+      plan->clear_bytes = g.partials_off;
+      plan->grid = plan->grid ? g.units * v->ctas : 0;
+    }
     const cudaError_t e = cudaMemsetAsync(workspace, 0, plan->clear_bytes, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) {
       free(plan);

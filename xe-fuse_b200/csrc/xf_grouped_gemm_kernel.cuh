@@ -53,6 +53,11 @@ struct alignas(64) Params {
   int d_f32, pair, vec_d;
   int* status;
   long long wait_budget;
+  // Tiles whose K range several units share (split_kb > 0: see Split): one flag per epilogue warp and one
+  // slot of partial sums per CTA.
+  int split_kb;          // what sharing costs, in K blocks of one unit
+  int* flags;            // [grid][8], zero between launches
+  float4* partials;      // [grid][8 warps][columns of a warp / 4][32 lanes]
 };
 
 template <int KIND_, int BN_, int CTAS_>
@@ -112,10 +117,52 @@ __device__ __forceinline__ Tile decode(const Params& p, const int* first, const 
 struct Item {
   int tile, kb0, kb1;
 };
-struct Schedule {
-  int next_tile;
-  __device__ __forceinline__ bool next(const Params& p, const int* first, int units, Item& it) {
-    if (next_tile >= ptx::uniform(first[p.G])) return false;
+
+// The work items of one unit (a CTA, or a pair of them).  Unit u takes the whole tiles u, u + U, ... of the full
+// waves.  The R tiles of the last, partly filled wave are laid end to end, R * num_kb blocks, and cut into
+// equal ranges, one for each of `sharers` units, if that saves more than the exchange of partial sums
+// costs (split_kb).  A unit walks its range backwards and before its whole tiles: the piece at the
+// range's end, which may lack the tile's last blocks, is published at once; the piece at its start, which
+// then has the tile's last block, collects what the units below it published.  So a unit only ever waits for
+// units of lower index, which never wait before they publish: the wait ends whatever else runs on the GPU.
+struct Split {
+  int whole;        // tiles of full waves
+  int sharers;      // units that share the others
+  int lo, hi;       // this unit's range
+  // Start of unit u's range: blocks * u / sharers, in 32 bits (a 64-bit division is a call, and what lives in
+  // registers around it is spilled).  The host keeps num_kb below 2^20.
+  __device__ __forceinline__ static int bound(unsigned blocks, unsigned sharers, unsigned u) {
+    const unsigned q = blocks / sharers;
+    return static_cast<int>(q * u + (blocks - q * sharers) * u / sharers);
+  }
+  __device__ __forceinline__ void set(const Params& p, int tiles, int unit, int units) {
+    const int rest = tiles % units;
+    whole = tiles;
+    sharers = lo = hi = 0;
+    if (p.split_kb == 0 || rest == 0) return;
+    // at least 4 blocks for each unit, and at most 8 units for each tile (they are summed one by one)
+    const int n = min(min(units, 8 * rest), rest * p.num_kb / 4);
+    if (n <= rest || (n - rest) * static_cast<long long>(p.num_kb) <= static_cast<long long>(p.split_kb) * n) return;
+    sharers = n;
+    whole = tiles - rest;
+    if (unit >= n) return;
+    lo = bound(rest * p.num_kb, n, unit);
+    hi = bound(rest * p.num_kb, n, unit + 1);
+  }
+};
+// A role's walk over them; the split stays in shared memory, out of the role's registers.
+struct Walk {
+  int next_tile, pos;
+  __device__ __forceinline__ bool next(const Params& p, const Split& s, int units, Item& it) {
+    if (pos > s.lo) {
+      const int t = (pos - 1) / p.num_kb, start = t * p.num_kb;
+      it.tile = ptx::uniform(s.whole + t);
+      it.kb1 = ptx::uniform(pos - start);
+      it.kb0 = ptx::uniform(max(s.lo - start, 0));
+      pos = max(s.lo, start);
+      return true;
+    }
+    if (next_tile >= ptx::uniform(s.whole)) return false;
     it.tile = next_tile;
     it.kb0 = 0;
     it.kb1 = p.num_kb;
@@ -139,6 +186,9 @@ __device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float(stat
 __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t x, uint64_t f) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(f));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, float lo, float hi) {
+  return pair_of(__float_as_uint(lo_of(a) + lo), __float_as_uint(hi_of(a) + hi));
 }
 // acc += r * f for the 16 words r of a TMEM slice, two columns per instruction; f holds the factor twice.
 __device__ __forceinline__ void scale_add(uint64_t* acc, const uint4 (&r)[4], uint64_t f) {
@@ -199,6 +249,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   uint64_t* tempty_bar = tfull_bar + NBUF;       // [NBUF]   accumulator read out (the leader CTA's is used)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + NBUF);
   int* first = reinterpret_cast<int*>(staging + 8 * C::STG_BYTES + C::BAR_BYTES);   // [G + 1] first tile of a group
+  Split* split = reinterpret_cast<Split*>(tmem_slot + 1);
   int* grow = first + kMaxGroups + 1;            // [G][2] first row, rows
 
   const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -254,7 +305,10 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       if (g < p.G) first[g + 1] = base + n;
       base += __shfl_sync(0xffffffffu, n, 31);
     }
-    if (lane == 0) first[0] = 0;
+    if (lane == 0) {
+      first[0] = 0;
+      split->set(p, base, unit, units);
+    }
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -264,7 +318,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   }
   ptx::tc_fence_after();
   const uint32_t tmem = ptx::uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
-  Schedule sched = {unit};
+  Walk sched = {unit, ptx::uniform(split->hi)};
   Item it;
   ptx::Waiter<Params> w = {p, false};
 
@@ -277,7 +331,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
     // ------------------------------------------------------------------ TMA producer
     int stage = 0;
     uint32_t phase = 0;
-    while (sched.next(p, first, units, it)) {
+    while (sched.next(p, *split, units, it)) {
       const Tile x = decode<C>(p, first, grow, it.tile);
       // rows of A that this CTA needs, and the bytes that both CTAs of a pair load
       uint32_t bytes = 0;
@@ -338,7 +392,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       const uint32_t tfull0 = ptx::smem_u32(tfull_bar), tempty0 = ptx::smem_u32(tempty_bar);
       int stage = 0, buf = 0;
       uint32_t phase = 0, tphase = 0;
-      while (sched.next(p, first, units, it)) {
+      while (sched.next(p, *split, units, it)) {
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           const bool fresh = KIND == KIND_E4M3 || kb == it.kb0;          // starts an accumulator
           const bool done = KIND == KIND_E4M3 || kb + 1 == it.kb1;       // and completes it
@@ -406,7 +460,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         }
       }
     };
-    bool more = sched.next(p, first, units, it);
+    bool more = sched.next(p, *split, units, it);
     if (more) enter();
     while (more) {
       uint64_t sum[NC / 2];                    // columns 2 i and 2 i + 1
@@ -467,6 +521,40 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
           take(f1);
         }
       }
+      if (it.kb1 < p.num_kb) {
+        // Not the tile's last blocks: the sums go to this CTA's slot, in a layout in which a warp's lanes are side by side.
+        float4* slot = p.partials + (static_cast<size_t>(blockIdx.x) * 8 + (warp - 4)) * (NC / 4) * 32 + lane;
+        if (live && lane < rows) {
+#pragma unroll
+          for (int i = 0; i < NC / 4; ++i)
+            slot[i * 32] = make_float4(lo_of(sum[2 * i]), hi_of(sum[2 * i]), lo_of(sum[2 * i + 1]), hi_of(sum[2 * i + 1]));
+        }
+        __syncwarp();
+        if (live && lane == 0) {
+          __threadfence();
+          *reinterpret_cast<volatile int*>(p.flags + blockIdx.x * 8 + (warp - 4)) = 1;
+        }
+        live = false;
+      } else if (it.kb0 > 0 && live) {
+        // The tile's last blocks: the units below hold the rest, nearest first, down to the one with block 0.
+        const int blocks = (first[p.G] - split->whole) * p.num_kb, start = (it.tile - split->whole) * p.num_kb;
+        for (int u = unit - 1;; --u) {
+          const int cta = u * CTAS + static_cast<int>(rank);
+          int* flag = p.flags + cta * 8 + (warp - 4);
+          w.wait_flag(flag, DEV_TIMEOUT_SPLIT_PARTIALS);
+          // lanes without a row add what the first lane's holds: no branch around 128 registers
+          const float4* slot = p.partials + (static_cast<size_t>(cta) * 8 + (warp - 4)) * (NC / 4) * 32 + (lane < rows ? lane : 0);
+#pragma unroll
+          for (int i = 0; i < NC / 4; ++i) {
+            const float4 f = __ldcg(slot + i * 32);
+            sum[2 * i] = add2(sum[2 * i], f.x, f.y);
+            sum[2 * i + 1] = add2(sum[2 * i + 1], f.z, f.w);
+          }
+          __syncwarp();
+          if (lane == 0) *reinterpret_cast<volatile int*>(flag) = 0;
+          if (Split::bound(blocks, split->sharers, u) <= start) break;
+        }
+      }
       const int wcol = OUT == OUT_PAIR_BF16 || OUT == OUT_PAIR_F32 ? col >> 1 : col, drow = x.row0 + roff;
       // 64 bytes of each row at a time, through the warp's staging buffers in turn
       constexpr bool F32 = OUT == OUT_F32 || OUT == OUT_PAIR_F32, PAIR = OUT == OUT_PAIR_BF16 || OUT == OUT_PAIR_F32;
@@ -506,7 +594,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         if (lane == 0) ptx::tma_store_commit();
         stg_at = stg_at + 1 == C::STG_BUFS ? 0 : stg_at + 1;
       }
-      more = sched.next(p, first, units, it);
+      more = sched.next(p, *split, units, it);
       if (more) enter();
     }
     if (lane == 0) ptx::tma_store_wait_read<0>();   // the staging buffers have been read before the CTA goes

@@ -165,6 +165,9 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
   return true;
 }
 
+// A value that is the same in all lanes, known as such to the compiler.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // A role's bounded waits.  One that runs out writes its code to the status word and lets the role go on
 // without waiting again for long: the launch is lost, but every role still walks its whole list and control
 // flow does not depend on a wait's outcome (a loop that a wait may leave keeps its counters, and with them
@@ -181,10 +184,19 @@ struct Waiter {
       lost = true;
     }
   }
+  // Until another CTA has set a flag in global memory; by a converged warp (a loop in one lane only made
+  // the compiler spill what lives in registers around it).
+  __device__ __forceinline__ void wait_flag(const int* flag, int code) {
+    const long long t0 = clock64();
+    while (__shfl_sync(0xffffffffu, ld_acquire_gpu(flag), 0) == 0) {
+      if (uniform(clock64() - t0 > (lost ? 0 : p.wait_budget))) {
+        if (p.status) atomicCAS(p.status, 0, code);
+        lost = true;
+        break;
+      }
+    }
+  }
 };
-
-// A value that is the same in all lanes, known as such to the compiler.
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // Read-only 4-byte load that the compiler may not move to where its value is used.
 __device__ __forceinline__ float ld_early(const float* p) {

@@ -140,8 +140,10 @@ struct Split {
     whole = tiles;
     sharers = lo = hi = 0;
     if (p.split_kb == 0 || rest == 0) return;
-    // at least 4 blocks for each unit, and at most 8 units for each tile (they are summed one by one)
-    const int n = min(min(units, 8 * rest), rest * p.num_kb / 4);
+    // At least 4 blocks for each unit, at most 8 units for each tile (they are summed one by one), and where
+    // two or more units go to a tile the same number to each: a range that touches two tiles adds a sharer.
+    int n = min(min(units, 8 * rest), rest * p.num_kb / 4);
+    if (n >= 2 * rest) n -= n % rest;
     if (n <= rest || (n - rest) * static_cast<long long>(p.num_kb) <= static_cast<long long>(p.split_kb) * n) return;
     sharers = n;
     whole = tiles - rest;
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   }
   // Everything above touched neither global memory nor what the previous kernel of the stream writes.
   ptx::griddep_launch_dependents();
-  ptx::griddep_wait();
+  if (p.offsets) ptx::griddep_wait();
 
   // Rows of each group, clamped to the rows there are: whatever the offsets hold, no tile leaves A and D.
   for (int g = threadIdx.x; g < p.G; g += 384) {
@@ -317,6 +319,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
     ptx::cluster_wait();
   }
   ptx::tc_fence_after();
+  if (!p.offsets) ptx::griddep_wait();
   const uint32_t tmem = ptx::uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
   Walk sched = {unit, ptx::uniform(split->hi)};
   Item it;
@@ -538,10 +541,14 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       } else if (it.kb0 > 0 && live) {
         // The tile's last blocks: the units below hold the rest, nearest first, down to the one with block 0.
         const int blocks = (first[p.G] - split->whole) * p.num_kb, start = (it.tile - split->whole) * p.num_kb;
-        for (int u = unit - 1;; --u) {
-          const int cta = u * CTAS + static_cast<int>(rank);
-          int* flag = p.flags + cta * 8 + (warp - 4);
-          w.wait_flag(flag, DEV_TIMEOUT_SPLIT_PARTIALS);
+        int count = 1;
+        while (Split::bound(blocks, split->sharers, unit - count) > start) ++count;
+        // one lane for each of them, all flags at once; then their sums, nearest unit first
+        int* flag = p.flags + ((unit - 1 - min(lane, count - 1)) * CTAS + static_cast<int>(rank)) * 8 + (warp - 4);
+        w.wait_flags(flag, DEV_TIMEOUT_SPLIT_PARTIALS);
+#pragma unroll 1
+        for (int u = 1; u <= count; ++u) {
+          const int cta = (unit - u) * CTAS + static_cast<int>(rank);
           // lanes without a row add what the first lane's holds: no branch around 128 registers
           const float4* slot = p.partials + (static_cast<size_t>(cta) * 8 + (warp - 4)) * (NC / 4) * 32 + (lane < rows ? lane : 0);
 #pragma unroll
@@ -550,10 +557,9 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
             sum[2 * i] = add2(sum[2 * i], f.x, f.y);
             sum[2 * i + 1] = add2(sum[2 * i + 1], f.z, f.w);
           }
-          __syncwarp();
-          if (lane == 0) *reinterpret_cast<volatile int*>(flag) = 0;
-          if (Split::bound(blocks, split->sharers, u) <= start) break;
         }
+        __syncwarp();
+        if (lane < count) *reinterpret_cast<volatile int*>(flag) = 0;   // for the next launch
       }
       const int wcol = OUT == OUT_PAIR_BF16 || OUT == OUT_PAIR_F32 ? col >> 1 : col, drow = x.row0 + roff;
       // 64 bytes of each row at a time, through the warp's staging buffers in turn

@@ -184,11 +184,11 @@ struct Waiter {
       lost = true;
     }
   }
-  // Until another CTA has set a flag in global memory; by a converged warp (a loop in one lane only made
-  // the compiler spill what lives in registers around it).
-  __device__ __forceinline__ void wait_flag(const int* flag, int code) {
+  // Until other CTAs have set the flags that the lanes name; by a converged warp (a loop in one lane only
+  // made the compiler spill what lives in registers around it).
+  __device__ __forceinline__ void wait_flags(const int* flag, int code) {
     const long long t0 = clock64();
-    while (__shfl_sync(0xffffffffu, ld_acquire_gpu(flag), 0) == 0) {
+    while (!__all_sync(0xffffffffu, ld_acquire_gpu(flag) != 0)) {
       if (uniform(clock64() - t0 > (lost ? 0 : p.wait_budget))) {
         if (p.status) atomicCAS(p.status, 0, code);
         lost = true;

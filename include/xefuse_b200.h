@@ -374,22 +374,27 @@ XF_API xf_status xf_ve_dequant_rotary(void* out, const int32_t* acc, const float
  * scale[m * scale_row_stride + b * scale_blk_stride].  Maxima are floored at 2^-100 times the row's
  * rstd, so zeros get zero codes and a finite scale; a NaN or an infinity makes the scale of its block
  * NaN or infinite.  Pitches in elements, any value from the row's width up and any alignment; 16-byte
- * aligned rows are faster.  N (d) up to 2^20.  M == 0 is an empty call.  All asynchronous on
+ * aligned rows are faster.  N up to 2^20.  M == 0 is an empty call.  All asynchronous on
  * `stream`, of the current device; no workspace.
  */
+typedef struct xf_quantize_desc {
+  void* out;                   /* [M][N] int8 or e4m3 */
+  float* scale;
+  const void* input;           /* bf16 [M][N]; xf_act_mul_quantize: [M][2N] */
+  const void* residual;        /* bf16 [M][N] or NULL; the norm only, like the next two */
+  void* residual_out;          /* bf16 [M][N]; may be residual: the stream updated in place */
+  const void* weight;          /* bf16 [N] or NULL (ones) */
+  int64_t ld_out, scale_row_stride, scale_blk_stride, ld_in, ld_res, ld_res_out;
+  int32_t out_dtype, M, N;
+  float eps;                   /* the norm only */
+  int32_t gelu;                /* the gate only: 0 SiLU, 1 erf-GeLU */
+  int32_t pad_;
+} xf_quantize_desc;
 /* v = RMSNorm(h) * weight with h = input, or, where residual is given, h = bf16(input + residual), which
- * is written to residual_out (may be residual itself: the stream updated in place).  The mean square is
- * taken over the rounded h.  weight bf16 [N] or NULL (ones). */
-XF_API xf_status xf_rms_norm_quantize(void* out, int out_dtype, int64_t ld_out, float* scale,
-                                      int64_t scale_row_stride, int64_t scale_blk_stride,
-                                      const void* input, int64_t ld_in, const void* residual,
-                                      int64_t ld_res, void* residual_out, int64_t ld_res_out,
-                                      const void* weight, int M, int N, float eps, void* stream);
-/* v[m,i] = act(input[m,i]) * input[m,d+i]; input bf16 [M,2d]; gelu=0 SiLU, 1 erf-GeLU. */
-XF_API xf_status xf_act_mul_quantize(void* out, int out_dtype, int64_t ld_out, float* scale,
-                                     int64_t scale_row_stride, int64_t scale_blk_stride,
-                                     const void* input, int64_t ld_in, int d, int M, int gelu,
-                                     void* stream);
+ * is written to residual_out.  The mean square is taken over the rounded h. */
+XF_API xf_status xf_rms_norm_quantize(const xf_quantize_desc* desc, void* stream);
+/* v[m,i] = act(input[m,i]) * input[m,N+i]. */
+XF_API xf_status xf_act_mul_quantize(const xf_quantize_desc* desc, void* stream);
 
 /*
  * Products of ragged row groups, each with its own weight (the experts of a mixture, rows sorted by

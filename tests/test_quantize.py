@@ -8,7 +8,6 @@ Tolerances, counted before the first run (u = 2^-24, the rounding of one fp32 op
  * gate: __expf(x) is within 2 + 1.173 |x| ulp (2 u each), which a sigmoid passes on at most once;
    the sum, the division (2 ulp) and the product with `up` add 8 u.  erf in gelu is within 1.5e-7 of 1 + erf.
 """
-import ctypes as C
 import math
 
 import pytest
@@ -206,37 +205,53 @@ def test_no_rows_and_other_streams(capi, cuda):
 
 
 # ------------------------------------------------------------------ refusals: no GPU is touched
-def norm_args(**k):
-    a = dict(out=0x1000, dt=4, ldo=512, s=0x2000, sr=1, sb=8, i=0x3000, ldi=512, r=None, ldr=0, h=None, ldh=0, w=None, M=8,
-             N=512, eps=1e-6, st=None)
-    a.update(k)
-    return list(a.values())
+def desc(capi, **k):
+    """A packed xf_quantize_desc of a valid norm, with some fields changed."""
+    d = dict(out=0x1000, scale=0x2000, input=0x3000, residual=0, residual_out=0, weight=0, ld_out=512, scale_row=1, scale_blk=8,
+             ld_in=512, ld_res=0, ld_res_out=0, out_dtype=4, M=8, N=512, eps=1e-6, gelu=0, pad=0)
+    assert set(k) <= set(d)
+    return capi._QUANTIZE_DESC.pack(*{**d, **k}.values())
 
 
-@pytest.mark.parametrize("change,status", [
-    (dict(M=-1), 4), (dict(N=0), 4), (dict(dt=0), 2), (dict(out=None), 4), (dict(s=None), 4), (dict(i=None), 4),
-    (dict(ldi=511), 3), (dict(ldo=511), 3), (dict(sr=0), 3), (dict(sb=0), 3), (dict(N=(1 << 20) + 1), 5),
-    (dict(i=0x3001), 1), (dict(s=0x2002), 1), (dict(r=0x4000, ldr=512), 4), (dict(h=0x4000, ldh=512), 4),
-    (dict(r=0x4000, ldr=511, h=0x4000, ldh=512), 3), (dict(r=0x4001, ldr=512, h=0x4000, ldh=512), 1), (dict(w=0x5001), 1),
-])
+def test_packed_descriptor_is_the_headers(capi):
+    fields = "out scale input residual residual_out weight ld_out scale_row_stride scale_blk_stride ld_in ld_res " \
+             "ld_res_out out_dtype M N eps gelu pad_".split()
+    import os
+    header = open(os.path.join(os.path.dirname(capi.HERE), "include", "xefuse_b200.h")).read()
+    body = header[header.index("typedef struct xf_quantize_desc"):header.index("} xf_quantize_desc;")]
+    import re
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    names = [n.strip(" *") for line in re.findall(r"\b(?:void\*|float\*|int64_t|int32_t|float)\s+([^;]+);", body) for n in line.split(",")]
+    assert names == fields and capi._QUANTIZE_DESC.size == 120
+
+
+BAD = [(dict(M=-1), 4), (dict(N=0), 4), (dict(out_dtype=0), 2), (dict(out=0), 4), (dict(scale=0), 4), (dict(input=0), 4),
+       (dict(ld_in=511), 3), (dict(ld_out=511), 3), (dict(scale_row=0), 3), (dict(scale_blk=0), 3), (dict(N=(1 << 20) + 1), 5),
+       (dict(input=0x3001), 1), (dict(scale=0x2002), 1)]
+
+
+@pytest.mark.parametrize("change,status", BAD + [
+    (dict(residual=0x4000, ld_res=512), 4), (dict(residual_out=0x4000, ld_res_out=512), 4),
+    (dict(residual=0x4000, ld_res=511, residual_out=0x4000, ld_res_out=512), 3),
+    (dict(residual=0x4001, ld_res=512, residual_out=0x4000, ld_res_out=512), 1), (dict(weight=0x5001), 1)])
 def test_norm_refusals(capi, change, status):
-    assert capi.lib().xf_rms_norm_quantize(*norm_args(**change)) == status
+    assert capi.lib().xf_rms_norm_quantize(desc(capi, **change), None) == status
     assert capi.lib().xf_last_error_string()
 
 
-@pytest.mark.parametrize("change,status", [
-    (dict(M=-1), 4), (dict(d=0), 4), (dict(dt=3), 2), (dict(out=None), 4), (dict(ldi=1023), 3), (dict(ldo=511), 3),
-    (dict(d=(1 << 20) + 1), 5), (dict(i=0x3001), 1),
-])
+@pytest.mark.parametrize("change,status", BAD + [
+    (dict(ld_in=1023), 3), (dict(weight=0x5000, ld_in=1024), 4),
+    (dict(residual=0x4000, ld_res=512, residual_out=0x4000, ld_res_out=512, ld_in=1024), 4)])
 def test_act_refusals(capi, change, status):
-    a = dict(out=0x1000, dt=4, ldo=512, s=0x2000, sr=1, sb=8, i=0x3000, ldi=1024, d=512, M=8, gelu=0, st=None)
-    a.update(change)
-    assert capi.lib().xf_act_mul_quantize(*a.values()) == status
+    assert capi.lib().xf_act_mul_quantize(desc(capi, **{"ld_in": 1024, **change}), None) == status
 
 
 def test_empty_calls(capi):
-    assert capi.lib().xf_rms_norm_quantize(*norm_args(M=0, out=None, i=None, s=None)) == 0
-    assert capi.lib().xf_act_mul_quantize(None, 4, 512, None, 1, 8, None, 1024, 512, 0, 0, None) == 0
+    empty = desc(capi, M=0, out=0, input=0, scale=0)
+    assert capi.lib().xf_rms_norm_quantize(empty, None) == 0
+    assert capi.lib().xf_act_mul_quantize(empty, None) == 0
+    assert capi.lib().xf_rms_norm_quantize(None, None) == 4
+    assert capi.lib().xf_act_mul_quantize(None, None) == 4
 
 
 def test_wrapper_refusals(capi, monkeypatch):

@@ -6,6 +6,7 @@ fallback: if the shared library is missing or an entry returns an error, XfError
 """
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libxefuse_b200.so")
@@ -158,9 +159,8 @@ def lib():
     L.xf_ve_rotary_embedding.argtypes = [vp, vp, vp, i32, i32, i32, i32, i32, vp]
     L.xf_ve_dequant_act_mul.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, vp]
     L.xf_ve_dequant_rotary.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, vp]
-    i64 = C.c_int64
-    L.xf_rms_norm_quantize.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, vp, i64, vp, i64, vp, i32, i32, f32, vp]
-    L.xf_act_mul_quantize.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, i32, i32, i32, vp]
+    L.xf_rms_norm_quantize.argtypes = [C.c_char_p, vp]     # a packed xf_quantize_desc
+    L.xf_act_mul_quantize.argtypes = [C.c_char_p, vp]
     L.xf_grouped_gemm_can_implement.argtypes = [C.POINTER(XfGroupedGemmDesc)]
     L.xf_grouped_gemm_workspace_size.argtypes = [C.POINTER(XfGroupedGemmDesc), C.POINTER(C.c_size_t)]
     L.xf_grouped_gemm_plan_create.argtypes = [C.POINTER(XfGroupedGemmDesc), vp, vp, C.POINTER(vp)]
@@ -306,8 +306,8 @@ class GroupedGemmPlan:
         N = B.shape[-2] if b_nk else B.shape[-1]
         G = offsets.shape[0] - 1 if offsets is not None else 1
         lead = () if B.dim() == 2 else (G,)
-        _rows(A, "A", M, K, A.dtype)
-        _rows(D, "D", M, N if pair == "none" else N // 2, D.dtype)
+        lda = _rows(A, "A", (M, K), A.dtype)
+        ldd = _rows(D, "D", (M, N if pair == "none" else N // 2), D.dtype)
         if tuple(B.shape) != lead + ((N, K) if b_nk else (K, N)) or (B.shape[-1] > 1 and B.stride(-1) != 1):
             raise XfError(3, f"B: {tuple(B.shape)} with strides {B.stride()} does not fit A {tuple(A.shape)} and {G} groups")
         if offsets is not None and (offsets.dtype != torch.int32 or offsets.dim() != 1 or not offsets.is_contiguous()):
@@ -316,11 +316,12 @@ class GroupedGemmPlan:
         d.dtype_ab, d.dtype_d = _torch_dtype_code(A), _torch_dtype_code(D)
         d.M, d.N, d.K, d.num_groups = M, N, K, G
         d.group_offsets = offsets.data_ptr() if offsets is not None else None
-        d.A, d.lda = A.data_ptr(), _pitch(A)
-        d.B, d.ldb, d.batch_b = B.data_ptr(), _pitch(B), (B.stride(0) if lead and G > 1 else 0)
+        d.A, d.lda = A.data_ptr(), lda
+        d.B, d.ldb = B.data_ptr(), (B.stride(-2) if B.shape[-2] > 1 else -(-B.shape[-1] // 16) * 16)
+        d.batch_b = (B.stride(0) if lead and G > 1 else 0)
         d.b_layout = B_NK if b_nk else B_KN
         d.pair = PAIR[pair]
-        d.D, d.ldd = D.data_ptr(), _pitch(D)
+        d.D, d.ldd = D.data_ptr(), ldd
         d.flags = flags
         if A.dtype == torch.float8_e4m3fn and (scale_a is None or scale_b is None):
             raise XfError(4, "float8_e4m3fn operands need scale_a and scale_b")
@@ -363,11 +364,6 @@ class GroupedGemmPlan:
             self.close()
         except Exception:
             pass
-
-
-def _pitch(t):
-    """Row pitch of a matrix (or stack of matrices) with contiguous columns; a single row's is of no use."""
-    return t.stride(-2) if t.shape[-2] > 1 else -(-t.shape[-1] // 16) * 16
 
 
 def cluster_capacity(dtype_code=DT_BF16):
@@ -497,14 +493,20 @@ def ve_dequant_rotary(out, acc, scale_token, scale_channel, cos_sin):
 
 
 # ---- row passes with an 8-bit output --------------------------------------------------------------
-def _rows(t, what, M, N, dtype):
-    """Checks a [M, N] tensor with contiguous columns and returns (pointer, row pitch)."""
+# xf_quantize_desc, packed in one step: these calls are a few microseconds on the GPU, and filling a ctypes
+# structure (or passing 17 arguments) takes longer than that.
+_QUANTIZE_DESC = struct.Struct("=6Q6q3ifii")
+
+
+def _rows(t, what, shape, dtype):
+    """Checks a matrix with contiguous columns and returns its row pitch."""
     if t.dtype != dtype:
         raise XfError(2, f"{what}: expected {dtype}, got {t.dtype}")
-    if tuple(t.shape) != (M, N) or (N > 1 and t.stride(1) != 1):
-        raise XfError(3, f"{what}: expected a [{M}, {N}] tensor with contiguous columns, got "
-                         f"{tuple(t.shape)} with strides {t.stride()}")
-    return t.data_ptr(), (t.stride(0) if M > 1 else max(t.stride(0), N))
+    st = t.stride()
+    if t.shape != shape or (st[1] != 1 and shape[1] > 1):
+        raise XfError(3, f"{what}: expected a {tuple(shape)} tensor with contiguous columns, got "
+                         f"{tuple(t.shape)} with strides {st}")
+    return st[0] if shape[0] > 1 else -(-shape[1] // 16) * 16    # a single row's pitch is of no use
 
 
 def _on_current_device(*tensors):
@@ -515,22 +517,23 @@ def _on_current_device(*tensors):
             raise XfError(4, f"tensor on {t.device}, but cuda:{cur} is the current device")
 
 
-def _scales(scale, dtype_code, M, N):
-    """Pointer and strides of the scales of an 8-bit [M, N] output."""
+def _codes(out, scale):
+    """(output type, row stride, block stride of the scales) of an 8-bit [M, N] output."""
     import torch
-    shape = (M,) if dtype_code == DT_S8 else (M, -(-N // 128))
-    if scale.dtype != torch.float32 or tuple(scale.shape) != shape:
-        raise XfError(3, f"scale: expected float32 {shape}, got {scale.dtype} {tuple(scale.shape)}")
-    # a dimension of one has no meaningful stride
-    return (scale.data_ptr(), scale.stride(0) if M > 1 else 1,
-            scale.stride(1) if dtype_code == DT_E4M3 and N > 128 else 1)
-
-
-def _code_dtype(out):
-    import torch
-    if out.dtype not in (torch.int8, torch.float8_e4m3fn):
+    M, N = out.shape
+    st = scale.stride()
+    if scale.dtype != torch.float32:
+        raise XfError(2, f"scale: expected float32, got {scale.dtype}")
+    if out.dtype == torch.float8_e4m3fn:
+        if scale.shape != (M, -(-N // 128)):
+            raise XfError(3, f"scale: expected {(M, -(-N // 128))}, got {tuple(scale.shape)}")
+        # a dimension of one has no meaningful stride
+        return DT_E4M3, st[0] if M > 1 else 1, st[1] if N > 128 else 1
+    if out.dtype != torch.int8:
         raise XfError(2, f"out: int8 or float8_e4m3fn, got {out.dtype}")
-    return DT_S8 if out.dtype == torch.int8 else DT_E4M3
+    if scale.shape != (M,):
+        raise XfError(3, f"scale: expected {(M,)}, got {tuple(scale.shape)}")
+    return DT_S8, st[0] if M > 1 else 1, 1
 
 
 def rms_norm_quantize(out, scale, inp, weight=None, residual=None, residual_out=None, eps=1e-6):
@@ -538,32 +541,40 @@ def rms_norm_quantize(out, scale, inp, weight=None, residual=None, residual_out=
     place when that is None).  out int8 with scale [M], or float8_e4m3fn with scale [M, ceil(N/128)] of any
     strides (the block-scaled products read fastest with the rows side by side: torch.empty(blocks, M).t())."""
     import torch
-    M, N = inp.shape
-    code = _code_dtype(out)
-    if residual is not None and residual_out is None:
-        residual_out = residual
+    shape, bf16 = inp.shape, torch.bfloat16
+    M, N = shape
     _on_current_device(out, scale, inp, weight, residual, residual_out)
-    if weight is not None and (weight.dtype != torch.bfloat16 or tuple(weight.shape) != (N,) or not weight.is_contiguous()):
+    code, sr, sb = _codes(out, scale)
+    il, ol = _rows(inp, "inp", shape, bf16), _rows(out, "out", shape, out.dtype)
+    rp = hp = rl = hl = 0
+    if residual is not None:
+        if residual_out is None:
+            residual_out = residual
+        rp, rl = residual.data_ptr(), _rows(residual, "residual", shape, bf16)
+        hp, hl = residual_out.data_ptr(), _rows(residual_out, "residual_out", shape, bf16)
+    if weight is not None and (weight.dtype != bf16 or weight.shape != (N,) or not weight.is_contiguous()):
         raise XfError(3, f"weight: expected contiguous bfloat16 [{N}], got {weight.dtype} {tuple(weight.shape)}")
-    ip, il = _rows(inp, "inp", M, N, torch.bfloat16)
-    op, ol = _rows(out, "out", M, N, out.dtype)
-    rp, rl = _rows(residual, "residual", M, N, torch.bfloat16) if residual is not None else (None, 0)
-    hp, hl = _rows(residual_out, "residual_out", M, N, torch.bfloat16) if residual is not None else (None, 0)
-    sp, sr, sb = _scales(scale, code, M, N)
-    check(lib().xf_rms_norm_quantize(op, code, ol, sp, sr, sb, ip, il, rp, rl, hp, hl,
-                                     weight.data_ptr() if weight is not None else None, M, N, eps, _stream()))
+    status = lib().xf_rms_norm_quantize(
+        _QUANTIZE_DESC.pack(out.data_ptr(), scale.data_ptr(), inp.data_ptr(), rp, hp,
+                            weight.data_ptr() if weight is not None else 0, ol, sr, sb, il, rl, hl, code, M, N, eps, 0, 0),
+        _stream())
+    if status:
+        check(status)
 
 
 def act_mul_quantize(out, scale, inp, gelu=False):
     """out, scale = 8-bit act(inp[:, :d]) * inp[:, d:]; inp [M, 2d]; out and scale as in rms_norm_quantize."""
     import torch
-    M, d = out.shape
-    code = _code_dtype(out)
+    shape = out.shape
+    M, d = shape
     _on_current_device(out, scale, inp)
-    ip, il = _rows(inp, "inp", M, 2 * d, torch.bfloat16)
-    op, ol = _rows(out, "out", M, d, out.dtype)
-    sp, sr, sb = _scales(scale, code, M, d)
-    check(lib().xf_act_mul_quantize(op, code, ol, sp, sr, sb, ip, il, d, M, 1 if gelu else 0, _stream()))
+    code, sr, sb = _codes(out, scale)
+    il, ol = _rows(inp, "inp", (M, 2 * d), torch.bfloat16), _rows(out, "out", shape, out.dtype)
+    status = lib().xf_act_mul_quantize(
+        _QUANTIZE_DESC.pack(out.data_ptr(), scale.data_ptr(), inp.data_ptr(), 0, 0, 0, ol, sr, sb, il, 0, 0, code, M, d,
+                            0.0, 1 if gelu else 0, 0), _stream())
+    if status:
+        check(status)
 
 
 def reduce_partials_rsqrt(partials, rstd, M, N, L=1, eps=1e-6):

@@ -571,15 +571,19 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         const int c = wcol + u * (F32 ? 16 : 32);
         if (c >= ncols || !live) break;
         float v[PAIR ? UNIT / 2 : UNIT];
+        const uint64_t* s = &sum[u * (UNIT / 2)];
+        if constexpr (!PAIR) {
 #pragma unroll
-        for (int i = 0; i < UNIT / 2; ++i) {
-          const uint64_t s = sum[u * (UNIT / 2) + i];
-          if constexpr (PAIR) {
-            v[i] = (p.pair == PAIR_SWIGLU ? silu_f(lo_of(s)) : gelu_f(lo_of(s))) * hi_of(s);
-          } else {
-            v[2 * i] = lo_of(s);
-            v[2 * i + 1] = hi_of(s);
+          for (int i = 0; i < UNIT / 2; ++i) {
+            v[2 * i] = lo_of(s[i]);
+            v[2 * i + 1] = hi_of(s[i]);
           }
+        } else if (p.pair == PAIR_SWIGLU) {      // the choice outside the loops: their elements interleave
+#pragma unroll
+          for (int i = 0; i < UNIT / 2; ++i) v[i] = silu_f(lo_of(s[i])) * hi_of(s[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < UNIT / 2; ++i) v[i] = gelu_f(lo_of(s[i])) * hi_of(s[i]);
         }
         uint32_t words[16];
 #pragma unroll

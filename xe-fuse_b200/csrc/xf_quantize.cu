@@ -27,6 +27,7 @@ namespace quantize {
 
 static const int kBlock = 128;        // columns that share a scale
 static const int kChunk = 8;          // columns a thread handles at a time: 16 bytes of bf16
+static const int kAhead = 4;          // chunks whose loads a thread of the norm has in flight
 static const float kFloor = 7.888609052210118e-31f;   // 2^-100
 
 struct Params {
@@ -182,38 +183,52 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const Params p) {
   const int lane = threadIdx.x & 31;
   float ss = 0.0f;
   uint32_t most = 0;
-  for (int c = threadIdx.x; c - lane < nchunk; c += blockDim.x) {
-    const int c0 = c * kChunk;
-    uint4 u = load_chunk(xr, c0, p.N, p.vec_in);
-    if (rr) {
-      const uint4 r = load_chunk(rr, c0, p.N, p.vec_res);
-      float a[8], b[8];
-      unpack(u, a);
-      unpack(r, b);
-      u = make_uint4(pack2(a[0] + b[0], a[1] + b[1]), pack2(a[2] + b[2], a[3] + b[3]),
-                     pack2(a[4] + b[4], a[5] + b[5]), pack2(a[6] + b[6], a[7] + b[7]));
-      store_chunk(hr, c0, p.N, p.vec_res, u);
-    }
-    float t[8];
-    unpack(u, t);
+  for (int base = threadIdx.x; base - lane < nchunk; base += kAhead * blockDim.x) {
+    // all loads of kAhead chunks before the first is used
+    uint4 x[kAhead], r[kAhead];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(t[i], t[i], ss);
-    if (p.weight) {
-      float w[8];
-      unpack(load_chunk(p.weight, c0, p.N, p.vec_w), w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] *= w[i];
+    for (int k = 0; k < kAhead; ++k) {
+      const int c = base + k * blockDim.x;
+      x[k] = r[k] = make_uint4(0, 0, 0, 0);
+      if (c < nchunk) {
+        x[k] = load_chunk(xr, c * kChunk, p.N, p.vec_in);
+        if (rr) r[k] = load_chunk(rr, c * kChunk, p.N, p.vec_res);
+      }
     }
-    const uint32_t mine = absmax_bits(t);
-    if (S8) {
-      most = max(most, mine);
-      if (p.row_bytes && c < nchunk) reinterpret_cast<uint4*>(dyn)[c] = u;
-    } else {
-      const uint32_t a = max16(mine);
-      uint32_t lo, hi;
-      codes_e4m3(t, floored(a), lo, hi);
-      store_codes(qr, c0, p.N, p.vec_out, lo, hi);
-      if ((lane & 15) == 0 && c < nchunk) reinterpret_cast<uint32_t*>(dyn)[c >> 4] = a;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int c = base + k * blockDim.x, c0 = c * kChunk;
+      if (c - lane >= nchunk) break;             // the whole warp
+      uint4 u = x[k];
+      if (rr) {
+        float a[8], b[8];
+        unpack(u, a);
+        unpack(r[k], b);
+        u = make_uint4(pack2(a[0] + b[0], a[1] + b[1]), pack2(a[2] + b[2], a[3] + b[3]),
+                       pack2(a[4] + b[4], a[5] + b[5]), pack2(a[6] + b[6], a[7] + b[7]));
+        store_chunk(hr, c0, p.N, p.vec_res, u);
+      }
+      float t[8];
+      unpack(u, t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(t[i], t[i], ss);
+      if (p.weight) {
+        float w[8];
+        unpack(load_chunk(p.weight, c0, p.N, p.vec_w), w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] *= w[i];
+      }
+      const uint32_t mine = absmax_bits(t);
+      if (S8) {
+        most = max(most, mine);
+        if (p.row_bytes && c < nchunk) reinterpret_cast<uint4*>(dyn)[c] = u;
+      } else {
+        const uint32_t a = max16(mine);
+        uint32_t lo, hi;
+        codes_e4m3(t, floored(a), lo, hi);
+        store_codes(qr, c0, p.N, p.vec_out, lo, hi);
+        if ((lane & 15) == 0 && c < nchunk) reinterpret_cast<uint32_t*>(dyn)[c >> 4] = a;
+      }
     }
   }
   block_sum_max(ss, most, red);
@@ -257,26 +272,37 @@ __device__ __forceinline__ void gated(const uint4& g, const uint4& u, float (&y)
   for (int i = 0; i < 8; ++i) y[i] = (GELU ? gelu_f(a[i]) : silu_f(a[i])) * b[i];
 }
 
-// e4m3: 16 lanes per block of 128 columns; nothing is shared beyond them.
+// e4m3: 16 lanes per block of 128 columns, two blocks in flight; nothing is shared beyond the lanes.
+static const int kBlocksEach = 2;
 template <bool GELU>
 __global__ void __launch_bounds__(256) act_mul_e4m3_kernel(const Params p, uint32_t nblk, unsigned long long total) {
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  const unsigned long long b0 = (static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x) >> 4;
-  const bool live = b0 < total;                     // 16 lanes agree; the others of the warp take part in its shuffles
-  const unsigned long long b = live ? b0 : 0;
-  const long long row = static_cast<long long>(b / nblk);
-  const int blk = static_cast<int>(b - row * nblk);
-  const int c0 = blk * kBlock + (threadIdx.x & 15) * kChunk;
-  const __nv_bfloat16* xr = p.in + row * p.ld_in;
-  float y[8];
-  gated<GELU>(load_chunk(xr, c0, p.N, p.vec_in), load_chunk(xr + p.N, c0, p.N, p.vec_res), y);
-  const float a = floored(max16(absmax_bits(y)));
-  if (!live) return;
-  uint32_t lo, hi;
-  codes_e4m3(y, a, lo, hi);
-  store_codes(p.out + row * p.ld_out, c0, p.N, p.vec_out, lo, hi);
-  if ((threadIdx.x & 15) == 0) p.scale[row * p.scale_row + blk * p.scale_blk] = __fdiv_rn(a, 448.0f);
+  const unsigned long long b0 = ((static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x) >> 4) * kBlocksEach;
+  uint4 g[kBlocksEach], u[kBlocksEach];
+  long long row[kBlocksEach];
+  int blk[kBlocksEach];
+  const int lane_col = (threadIdx.x & 15) * kChunk;
+#pragma unroll
+  for (int k = 0; k < kBlocksEach; ++k) {
+    const unsigned long long b = min(b0 + k, total - 1);   // all lanes of a warp take part in its shuffles
+    row[k] = static_cast<long long>(total <= 0xFFFFFFFFull ? static_cast<uint32_t>(b) / nblk : b / nblk);
+    blk[k] = static_cast<int>(b - row[k] * nblk);
+    const __nv_bfloat16* xr = p.in + row[k] * p.ld_in;
+    g[k] = load_chunk(xr, blk[k] * kBlock + lane_col, p.N, p.vec_in);
+    u[k] = load_chunk(xr + p.N, blk[k] * kBlock + lane_col, p.N, p.vec_res);
+  }
+#pragma unroll
+  for (int k = 0; k < kBlocksEach; ++k) {
+    float y[8];
+    gated<GELU>(g[k], u[k], y);
+    const float a = floored(max16(absmax_bits(y)));
+    if (b0 + k >= total) continue;
+    uint32_t lo, hi;
+    codes_e4m3(y, a, lo, hi);
+    store_codes(p.out + row[k] * p.ld_out, blk[k] * kBlock + lane_col, p.N, p.vec_out, lo, hi);
+    if (lane_col == 0) p.scale[row[k] * p.scale_row + blk[k] * p.scale_blk] = __fdiv_rn(a, 448.0f);
+  }
 }
 
 // int8: one block per row; the products wait in shared memory for the row's maximum, or are formed again
@@ -324,35 +350,64 @@ static int aligned(const void* p, long long pitch_bytes, int to) {
   return (reinterpret_cast<uintptr_t>(p) % to) == 0 && pitch_bytes % to == 0;
 }
 
-static xf_status check(const char* what, const void* out, int out_dtype, int64_t ld_out, const float* scale,
-                       int64_t scale_row, int64_t scale_blk, const void* in, int64_t ld_in, int in_cols, int M, int N) {
-  if (M < 0 || N <= 0) {
-    set_error("%s: extents must be positive (M=%d N=%d)", what, M, N);
+static xf_status check(const char* what, const xf_quantize_desc* d, long long in_cols) {
+  if (!d) {
+    set_error("%s: null descriptor", what);
     return XF_ERR_INVALID_PROBLEM;
   }
-  if (out_dtype != XF_DT_S8 && out_dtype != XF_DT_E4M3) {
-    set_error("%s: the output is int8 or e4m3 (got dtype %d)", what, out_dtype);
+  if (d->M < 0 || d->N <= 0) {
+    set_error("%s: extents must be positive (M=%d N=%d)", what, d->M, d->N);
+    return XF_ERR_INVALID_PROBLEM;
+  }
+  if (d->out_dtype != XF_DT_S8 && d->out_dtype != XF_DT_E4M3) {
+    set_error("%s: the output is int8 or e4m3 (got dtype %d)", what, d->out_dtype);
     return XF_ERR_INVALID_DATA_TYPE;
   }
-  if (N > (1 << 20)) {
-    set_error("%s: rows of at most %d columns (got %d)", what, 1 << 20, N);
+  if (d->N > (1 << 20)) {
+    set_error("%s: rows of at most %d columns (got %d)", what, 1 << 20, d->N);
     return XF_ERR_NOT_SUPPORTED;
   }
-  if (M == 0) return XF_SUCCESS;
-  if (!out || !scale || !in) {
+  if (d->M == 0) return XF_SUCCESS;
+  if (!d->out || !d->scale || !d->input) {
     set_error("%s: null pointer", what);
     return XF_ERR_INVALID_PROBLEM;
   }
-  if (ld_in < in_cols || ld_out < N || scale_row < 1 || (out_dtype == XF_DT_E4M3 && N > kBlock && scale_blk < 1)) {
-    set_error("%s: pitches too small (ld_in=%lld ld_out=%lld scale strides %lld, %lld; N=%d)", what, (long long)ld_in,
-              (long long)ld_out, (long long)scale_row, (long long)scale_blk, N);
+  if (d->ld_in < in_cols || d->ld_out < d->N || d->scale_row_stride < 1 ||
+      (d->out_dtype == XF_DT_E4M3 && d->N > kBlock && d->scale_blk_stride < 1)) {
+    set_error("%s: pitches too small (ld_in=%lld ld_out=%lld scale strides %lld, %lld; N=%d)", what,
+              (long long)d->ld_in, (long long)d->ld_out, (long long)d->scale_row_stride,
+              (long long)d->scale_blk_stride, d->N);
     return XF_ERR_INVALID_LAYOUT;
   }
-  if ((reinterpret_cast<uintptr_t>(in) & 1) || (reinterpret_cast<uintptr_t>(scale) & 3)) {
+  if (!d->residual != !d->residual_out) {
+    set_error("%s: residual and residual_out go together", what);
+    return XF_ERR_INVALID_PROBLEM;
+  }
+  if (d->residual && (d->ld_res < d->N || d->ld_res_out < d->N)) {
+    set_error("%s: residual pitches %lld, %lld smaller than N=%d", what, (long long)d->ld_res,
+              (long long)d->ld_res_out, d->N);
+    return XF_ERR_INVALID_LAYOUT;
+  }
+  auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  if (((bits(d->input) | bits(d->residual) | bits(d->residual_out) | bits(d->weight)) & 1) || (bits(d->scale) & 3)) {
     set_error("%s: pointers must be aligned to their element size", what);
     return XF_ERR_MISALIGNED_OPERAND;
   }
   return XF_SUCCESS;
+}
+
+static Params params_of(const xf_quantize_desc* d) {
+  Params p = {};
+  p.in = static_cast<const __nv_bfloat16*>(d->input); p.ld_in = d->ld_in;
+  p.residual = static_cast<const __nv_bfloat16*>(d->residual); p.ld_res = d->ld_res;
+  p.residual_out = static_cast<__nv_bfloat16*>(d->residual_out); p.ld_res_out = d->ld_res_out;
+  p.weight = static_cast<const __nv_bfloat16*>(d->weight);
+  p.out = static_cast<uint8_t*>(d->out); p.ld_out = d->ld_out;
+  p.scale = d->scale; p.scale_row = d->scale_row_stride; p.scale_blk = d->scale_blk_stride;
+  p.M = d->M; p.N = d->N; p.eps = d->eps;
+  p.vec_in = aligned(d->input, d->ld_in * 2, 16);
+  p.vec_out = aligned(d->out, d->ld_out, 8);
+  return p;
 }
 
 // Launches with programmatic stream serialization, like the products: the kernel waits for the previous
@@ -378,9 +433,11 @@ static xf_status launch(const char* what, void (*fn)(Args...), unsigned grid, un
   return XF_SUCCESS;
 }
 
-static unsigned row_threads(int N) {
-  const int chunks = (N + kChunk - 1) / kChunk;
-  const int t = (chunks + 31) / 32 * 32;
+// Threads for a row: one chunk each where there are few rows, kAhead where other rows keep the SM busy
+// (4096 x 8192: 1024 threads of one chunk 76 us, 256 of four XX us).
+static unsigned row_threads(int M, int N) {
+  const int chunks = (N + kChunk - 1) / kChunk, each = M >= 512 ? kAhead : 1;
+  const int t = ((chunks + each - 1) / each + 31) / 32 * 32;
   return t > 1024 ? 1024 : t;
 }
 
@@ -391,79 +448,49 @@ static const int kRowBytes = 47 * 1024;   // rows up to this size wait in shared
 
 extern "C" {
 
-xf_status xf_rms_norm_quantize(void* out, int out_dtype, int64_t ld_out, float* scale, int64_t scale_row_stride,
-                               int64_t scale_blk_stride, const void* input, int64_t ld_in, const void* residual,
-                               int64_t ld_res, void* residual_out, int64_t ld_res_out, const void* weight, int M,
-                               int N, float eps, void* stream) {
+xf_status xf_rms_norm_quantize(const xf_quantize_desc* d, void* stream) {
   using namespace xf;
   using namespace xf::quantize;
   const char* what = "rms_norm_quantize";
-  xf_status s = quantize::check(what, out, out_dtype, ld_out, scale, scale_row_stride, scale_blk_stride, input, ld_in, N, M, N);
-  if (s != XF_SUCCESS || M == 0) return s;
-  if (!residual != !residual_out) {
-    set_error("%s: residual and residual_out go together", what);
-    return XF_ERR_INVALID_PROBLEM;
-  }
-  if (residual && (ld_res < N || ld_res_out < N)) {
-    set_error("%s: residual pitches %lld, %lld smaller than N=%d", what, (long long)ld_res, (long long)ld_res_out, N);
-    return XF_ERR_INVALID_LAYOUT;
-  }
-  if ((reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(residual_out) |
-       reinterpret_cast<uintptr_t>(weight)) & 1) {
-    set_error("%s: pointers must be aligned to their element size", what);
-    return XF_ERR_MISALIGNED_OPERAND;
-  }
-  Params p = {};
-  p.in = static_cast<const __nv_bfloat16*>(input); p.ld_in = ld_in;
-  p.residual = static_cast<const __nv_bfloat16*>(residual); p.ld_res = ld_res;
-  p.residual_out = static_cast<__nv_bfloat16*>(residual_out); p.ld_res_out = ld_res_out;
-  p.weight = static_cast<const __nv_bfloat16*>(weight);
-  p.out = static_cast<uint8_t*>(out); p.ld_out = ld_out;
-  p.scale = scale; p.scale_row = scale_row_stride; p.scale_blk = scale_blk_stride;
-  p.M = M; p.N = N; p.eps = eps;
-  p.vec_in = aligned(input, ld_in * 2, 16);
-  p.vec_res = residual && aligned(residual, ld_res * 2, 16) && aligned(residual_out, ld_res_out * 2, 16);
-  p.vec_out = aligned(out, ld_out, 8);
-  p.vec_w = aligned(weight, 0, 16);
-  const int nchunk = (N + kChunk - 1) / kChunk;
-  if (out_dtype == XF_DT_E4M3)
-    return launch(what, rms_norm_kernel<false>, M, row_threads(N), (nchunk + 15) / 16 * sizeof(uint32_t), stream, p);
+  const xf_status s = quantize::check(what, d, d ? d->N : 0);
+  if (s != XF_SUCCESS || d->M == 0) return s;
+  Params p = params_of(d);
+  p.vec_res = d->residual && aligned(d->residual, d->ld_res * 2, 16) && aligned(d->residual_out, d->ld_res_out * 2, 16);
+  p.vec_w = aligned(d->weight, 0, 16);
+  const int nchunk = (d->N + kChunk - 1) / kChunk;
+  if (d->out_dtype == XF_DT_E4M3)
+    return launch(what, rms_norm_kernel<false>, d->M, row_threads(d->M, d->N), (nchunk + 15) / 16 * sizeof(uint32_t), stream, p);
   p.row_bytes = nchunk * 16 <= kRowBytes ? nchunk * 16 : 0;
-  return launch(what, rms_norm_kernel<true>, M, row_threads(N), p.row_bytes, stream, p);
+  return launch(what, rms_norm_kernel<true>, d->M, row_threads(d->M, d->N), p.row_bytes, stream, p);
 }
 
-xf_status xf_act_mul_quantize(void* out, int out_dtype, int64_t ld_out, float* scale, int64_t scale_row_stride,
-                              int64_t scale_blk_stride, const void* input, int64_t ld_in, int d, int M, int gelu,
-                              void* stream) {
+xf_status xf_act_mul_quantize(const xf_quantize_desc* d, void* stream) {
   using namespace xf;
   using namespace xf::quantize;
   const char* what = "act_mul_quantize";
-  const int in_cols = d > (1 << 20) ? d : 2 * d;
-  xf_status s = quantize::check(what, out, out_dtype, ld_out, scale, scale_row_stride, scale_blk_stride, input, ld_in, in_cols, M, d);
-  if (s != XF_SUCCESS || M == 0) return s;
-  Params p = {};
-  p.in = static_cast<const __nv_bfloat16*>(input); p.ld_in = ld_in;
-  p.out = static_cast<uint8_t*>(out); p.ld_out = ld_out;
-  p.scale = scale; p.scale_row = scale_row_stride; p.scale_blk = scale_blk_stride;
-  p.M = M; p.N = d;
-  p.vec_in = aligned(input, ld_in * 2, 16);
-  p.vec_res = aligned(p.in + d, ld_in * 2, 16);      // the second half of the row
-  p.vec_out = aligned(out, ld_out, 8);
-  if (out_dtype == XF_DT_E4M3) {
-    const uint32_t nblk = (d + kBlock - 1) / kBlock;
-    const unsigned long long total = static_cast<unsigned long long>(M) * nblk;
-    const unsigned long long grid = (total + 15) / 16;
+  const xf_status s = quantize::check(what, d, d ? 2LL * d->N : 0);
+  if (s != XF_SUCCESS || d->M == 0) return s;
+  if (d->residual || d->weight) {
+    set_error("%s: takes neither residual nor weight", what);
+    return XF_ERR_INVALID_PROBLEM;
+  }
+  Params p = params_of(d);
+  p.vec_res = aligned(p.in + d->N, d->ld_in * 2, 16);      // the second half of the row
+  if (d->out_dtype == XF_DT_E4M3) {
+    const uint32_t nblk = (d->N + kBlock - 1) / kBlock;
+    const unsigned long long total = static_cast<unsigned long long>(d->M) * nblk;
+    const unsigned long long grid = (total + 16 * kBlocksEach - 1) / (16 * kBlocksEach);
     if (grid > 0x7FFFFFFFull) {
-      set_error("%s: more than 2^31 thread blocks (M=%d d=%d)", what, M, d);
+      set_error("%s: more than 2^31 thread blocks (M=%d N=%d)", what, d->M, d->N);
       return XF_ERR_NOT_SUPPORTED;
     }
-    return gelu ? launch(what, act_mul_e4m3_kernel<true>, static_cast<unsigned>(grid), 256, 0, stream, p, nblk, total)
-                : launch(what, act_mul_e4m3_kernel<false>, static_cast<unsigned>(grid), 256, 0, stream, p, nblk, total);
+    return d->gelu ? launch(what, act_mul_e4m3_kernel<true>, static_cast<unsigned>(grid), 256, 0, stream, p, nblk, total)
+                   : launch(what, act_mul_e4m3_kernel<false>, static_cast<unsigned>(grid), 256, 0, stream, p, nblk, total);
   }
-  const int nchunk = (d + kChunk - 1) / kChunk;
+  const int nchunk = (d->N + kChunk - 1) / kChunk;
   p.row_bytes = nchunk * 32 <= kRowBytes ? nchunk * 32 : 0;
-  return gelu ? launch(what, act_mul_s8_kernel<true>, M, row_threads(d), p.row_bytes, stream, p)
-              : launch(what, act_mul_s8_kernel<false>, M, row_threads(d), p.row_bytes, stream, p);
+  return d->gelu ? launch(what, act_mul_s8_kernel<true>, d->M, row_threads(d->M, d->N), p.row_bytes, stream, p)
+                 : launch(what, act_mul_s8_kernel<false>, d->M, row_threads(d->M, d->N), p.row_bytes, stream, p);
 }
 
 }  // extern "C"

@@ -347,7 +347,9 @@ class GroupedGemmPlan:
         self.kernel_name = L_.xf_grouped_gemm_plan_kernel_name(self.handle).decode()
 
     def run(self, stream=None):
-        check(lib().xf_grouped_gemm_run(self.handle, stream if stream is not None else _stream()))
+        status = _lib.xf_grouped_gemm_run(self.handle, stream if stream is not None else _stream())
+        if status:
+            check(status)
 
     def device_status(self):
         code = C.c_int32(0)
@@ -374,8 +376,10 @@ def cluster_capacity(dtype_code=DT_BF16):
 
 
 def _stream():
+    """The current stream of the current device as a raw handle (without building a torch Stream object,
+    which takes 3 us, more than a launch)."""
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def sa_scale_rows(D, scale):

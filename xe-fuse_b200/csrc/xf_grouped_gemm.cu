@@ -128,9 +128,21 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
   }
   const int kind = d->dtype_ab == XF_DT_BF16 ? KIND_BF16 : KIND_E4M3;
   const Variant* v = nullptr;
-  // Pairs of CTAs on 256 x 256 tiles need half the operand bytes per multiplication of single CTAs on
-  // 128 x 128 tiles, which waste less on groups of few rows.
-  int ctas = d->M / d->num_groups > 128 ? 2 : 1;
+  // The tile: the lower estimate of waves x clocks per tile.  A K block takes about 780 clocks on a pair's
+  // 256 x 256 tile and 600 on a CTA's 128 x 128 tile with e4m3 (680 and 490 with bf16), the end of a tile 4500
+  // and 3000.  Pairs read half the operand bytes per multiplication; small tiles waste less on groups of few
+  // rows and spread better.  Rows of a group are taken to fill half of its last tile.
+  // Measured, pair against CTA: e4m3 4096 x 28672 x 4096 411 / 607 us, 777 x 5001 x 2000 37 / 27 us, bf16 with
+  // 8 groups 4096 x 4096 x 4096 125 / 146 us.
+  const int kblk = kind == KIND_BF16 ? 64 : 128;
+  auto clocks = [&](int ctas) {
+    const int side = 128 * ctas;
+    const double tiles_m = d->num_groups == 1 ? (d->M + side - 1) / side : static_cast<double>(d->M) / side + 0.5 * d->num_groups;
+    const double waves = tiles_m * ((d->N + side - 1) / side) * ctas / sms;
+    const double per_kb = kind == KIND_BF16 ? (ctas == 2 ? 680 : 490) : (ctas == 2 ? 780 : 600);
+    return (waves > 1 ? waves : 1) * ((d->K + kblk - 1) / kblk * per_kb + (ctas == 2 ? 4500 : 3000));
+  };
+  int ctas = clocks(2) < clocks(1) ? 2 : 1;
   if (d->flags & XF_FLAG_FORCE_1CTA) ctas = 1;
   else if (d->flags & XF_FLAG_FORCE_2CTA) ctas = 2;
   for (int i = 0; i < kTilesPerKind; ++i) {

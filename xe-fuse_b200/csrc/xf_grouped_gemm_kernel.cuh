@@ -30,6 +30,7 @@ namespace xf {
 namespace grouped {
 
 static const int kMaxGroups = 1024;
+static const int kTileList = 128;   // tiles of a unit that are looked up once, when the kernel starts
 enum : int { KIND_BF16 = 0, KIND_E4M3 = 2 };   // the KIND of ptx::umma
 // What a kernel instance writes.  One instance for each: the code of another form, never run, takes registers
 // that the loop over K blocks needs (spills there cost a sixth of the throughput).
@@ -73,15 +74,16 @@ struct Cfg {
   static constexpr int A_BYTES = 128 * 128;
   static constexpr int B_BYTES = BN_CTA * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 5;
+  static constexpr int STAGES = CTAS == 2 ? 4 : 5;
   static constexpr int NBUF = 512 / BN;                 // accumulators in TMEM
   static constexpr int NC = BN / 2;                     // columns per epilogue warp
   static constexpr bool SPLIT_REGS = NC == 128;
-  static constexpr int STG_BUFS = 3;                    // staging buffers per epilogue warp: 32 rows x 64 bytes
+  static constexpr int STG_BUFS = CTAS == 2 ? 4 : 2;    // staging buffers per epilogue warp: 32 rows x 64 bytes
   static constexpr int STG_BYTES = STG_BUFS * 2048;
   static constexpr int BAR_BYTES = 256;
   static constexpr int TAB_BYTES = (kMaxGroups + 1 + 2 * kMaxGroups) * 4;   // first tile, {first row, rows} of a group
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 8 * STG_BYTES + BAR_BYTES + TAB_BYTES;
+  static constexpr int LIST_BYTES = kTileList * 16;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 8 * STG_BYTES + BAR_BYTES + LIST_BYTES + TAB_BYTES;
   static_assert(BN_CTA == 128, "a CTA loads 128 columns of B");
   static_assert(NC % 64 == 0 && NC <= 128, "an epilogue warp's columns share one scale of B");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
@@ -154,8 +156,9 @@ struct Split {
 };
 // A role's walk over them; the split stays in shared memory, out of the role's registers.
 struct Walk {
-  int next_tile, pos;
+  int next_tile, pos, count;   // count: items taken, the place of the next one's tile in the list
   __device__ __forceinline__ bool next(const Params& p, const Split& s, int units, Item& it) {
+    ++count;
     if (pos > s.lo) {
       const int t = (pos - 1) / p.num_kb, start = t * p.num_kb;
       it.tile = ptx::uniform(s.whole + t);
@@ -211,28 +214,30 @@ __device__ __forceinline__ void stage_row64(uint8_t* buf, int lane, const uint32
     *reinterpret_cast<uint4*>(mine + ((j ^ sw) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
 }
 
-// Writes the first `rows` of the 32 staged rows to row-major global memory, four lanes per row: for row blocks
-// that end inside a group's last tile, and for rows that a tensor map cannot address.  ES: bytes per element.
+// Writes the first `rows` of the 32 staged rows to row-major global memory: for row blocks that end inside a
+// group's last tile, and for rows that a tensor map cannot address.  Four lanes per row with 16 bytes each
+// where rows allow it, else neighbouring lanes write neighbouring elements.  ES: bytes per element.
 template <int ES>
 __device__ __forceinline__ void copy_rows64(const uint8_t* buf, int lane, char* d, long long pitch, int rows, int col,
                                             int ncols, int vec) {
-  const int ch = lane & 3, c = col + ch * (16 / ES);
+  rows = min(rows, 32);
+  if (vec && col + 64 / ES <= ncols) {
+    const int ch = lane & 3;
 #pragma unroll 1
-  for (int r = lane >> 2; r < min(rows, 32); r += 8) {
-    if (c >= ncols) break;
-    const uint4 u = *reinterpret_cast<const uint4*>(buf + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4));
-    char* q = d + r * pitch + static_cast<long long>(c) * ES;
-    if (vec && c + 16 / ES <= ncols) {
-      *reinterpret_cast<uint4*>(q) = u;
-    } else {
-      const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int e = 0; e < 16 / ES; ++e) {
-        if (c + e >= ncols) break;
-        if (ES == 4) reinterpret_cast<uint32_t*>(q)[e] = x[e];
-        else reinterpret_cast<uint16_t*>(q)[e] = static_cast<uint16_t>(x[e >> 1] >> (16 * (e & 1)));
-      }
-    }
+    for (int r = lane >> 2; r < rows; r += 8)
+      *reinterpret_cast<uint4*>(d + r * pitch + static_cast<long long>(col) * ES + ch * 16) =
+          *reinterpret_cast<const uint4*>(buf + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4));
+    return;
+  }
+  constexpr int PER_ROW = 64 / ES, STEP = 32 / PER_ROW;   // elements of a row; rows a warp writes at a time
+  const int e = lane % PER_ROW;
+  if (col + e >= ncols) return;
+  char* q = d + static_cast<long long>(col + e) * ES;
+#pragma unroll 4
+  for (int r = lane / PER_ROW; r < rows; r += STEP) {
+    const uint8_t* s = buf + r * 64 + ((((e * ES) >> 4) ^ ((r >> 1) & 3)) << 4) + ((e * ES) & 15);
+    if (ES == 4) *reinterpret_cast<uint32_t*>(q + r * pitch) = *reinterpret_cast<const uint32_t*>(s);
+    else *reinterpret_cast<uint16_t*>(q + r * pitch) = *reinterpret_cast<const uint16_t*>(s);
   }
 }
 
@@ -250,7 +255,8 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   uint64_t* tfull_bar = bars + 2 * STAGES;       // [NBUF]   accumulator complete
   uint64_t* tempty_bar = tfull_bar + NBUF;       // [NBUF]   accumulator read out (the leader CTA's is used)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + NBUF);
-  int* first = reinterpret_cast<int*>(staging + 8 * C::STG_BYTES + C::BAR_BYTES);   // [G + 1] first tile of a group
+  Tile* list = reinterpret_cast<Tile*>(staging + 8 * C::STG_BYTES + C::BAR_BYTES);  // [kTileList] this unit's tiles
+  int* first = reinterpret_cast<int*>(list + kTileList);   // [G + 1] first tile of a group
   Split* split = reinterpret_cast<Split*>(tmem_slot + 1);
   int* grow = first + kMaxGroups + 1;            // [G][2] first row, rows
 
@@ -319,9 +325,20 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
     ptx::cluster_wait();
   }
   ptx::tc_fence_after();
+  // Where a unit takes several tiles, one thread looks up each of them now: every role would do it in turn,
+  // between tiles (64 groups, 16384 x 4096 x 2048: 275 -> 250 us; a single tile starts 1 us sooner without).
+  const int listed = ptx::uniform(first[p.G]) > 2 * units ? kTileList : 0;
+  if (listed) {
+    const int shared_tiles = split->hi > split->lo ? (split->hi - 1) / p.num_kb - split->lo / p.num_kb + 1 : 0;
+    for (int i = threadIdx.x; i < kTileList; i += 384) {
+      const int tile = i < shared_tiles ? split->whole + (split->hi - 1) / p.num_kb - i : unit + (i - shared_tiles) * units;
+      if (i < shared_tiles || tile < split->whole) list[i] = decode<C>(p, first, grow, tile);
+    }
+    __syncthreads();
+  }
   if (!p.offsets) ptx::griddep_wait();
   const uint32_t tmem = ptx::uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
-  Walk sched = {unit, ptx::uniform(split->hi)};
+  Walk sched = {unit, ptx::uniform(split->hi), 0};
   Item it;
   ptx::Waiter<Params> w = {p, false};
 
@@ -335,7 +352,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
     int stage = 0;
     uint32_t phase = 0;
     while (sched.next(p, *split, units, it)) {
-      const Tile x = decode<C>(p, first, grow, it.tile);
+      const Tile x = sched.count <= listed ? list[sched.count - 1] : decode<C>(p, first, grow, it.tile);
       // rows of A that this CTA needs, and the bytes that both CTAs of a pair load
       uint32_t bytes = 0;
       int boxes = 0;                             // of 32 rows; 4: one box of 128
@@ -448,7 +465,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
     const float* sb = nullptr;
     float a0 = 0.0f, b0 = 0.0f, a1 = 0.0f, b1 = 0.0f;
     auto enter = [&]() {
-      x = decode<C>(p, first, grow, it.tile);
+      x = sched.count <= listed ? list[sched.count - 1] : decode<C>(p, first, grow, it.tile);
       rows = x.rows - roff;
       col = x.n0 + half * NC;
       live = rows > 0 && col < p.N;
@@ -562,47 +579,55 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         if (lane < count) *reinterpret_cast<volatile int*>(flag) = 0;   // for the next launch
       }
       const int wcol = OUT == OUT_PAIR_BF16 || OUT == OUT_PAIR_F32 ? col >> 1 : col, drow = x.row0 + roff;
-      // 64 bytes of each row at a time, through the warp's staging buffers in turn
+      // 64 bytes of each row make a unit; two of them are staged before one fence hands them to the store engine
       constexpr bool F32 = OUT == OUT_F32 || OUT == OUT_PAIR_F32, PAIR = OUT == OUT_PAIR_BF16 || OUT == OUT_PAIR_F32;
       constexpr int UNIT = (F32 ? 16 : 32) * (PAIR ? 2 : 1);     // sums that make 64 bytes of D
+      constexpr int COLS = F32 ? 16 : 32;
+      constexpr int BOTH = NC / UNIT > 1 ? 2 : 1;
       const bool tma = p.vec_d && rows >= 32;    // a tensor map's box has 32 rows, all of this group
 #pragma unroll
-      for (int u = 0; u < NC / UNIT; ++u) {
-        const int c = wcol + u * (F32 ? 16 : 32);
-        if (c >= ncols || !live) break;
-        float v[PAIR ? UNIT / 2 : UNIT];
-        const uint64_t* s = &sum[u * (UNIT / 2)];
-        if constexpr (!PAIR) {
-#pragma unroll
-          for (int i = 0; i < UNIT / 2; ++i) {
-            v[2 * i] = lo_of(s[i]);
-            v[2 * i + 1] = hi_of(s[i]);
-          }
-        } else if (p.pair == PAIR_SWIGLU) {      // the choice outside the loops: their elements interleave
-#pragma unroll
-          for (int i = 0; i < UNIT / 2; ++i) v[i] = silu_f(lo_of(s[i])) * hi_of(s[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < UNIT / 2; ++i) v[i] = gelu_f(lo_of(s[i])) * hi_of(s[i]);
-        }
-        uint32_t words[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) words[i] = F32 ? __float_as_uint(v[i]) : pack_bf16(v[2 * i % (F32 ? 16 : 32)], v[(2 * i + 1) % (F32 ? 16 : 32)]);
-        uint8_t* b = stg + stg_at * 2048;
-        if (lane == 0) ptx::tma_store_wait_read<C::STG_BUFS - 1>();   // the buffer's last store has read it
+      for (int u0 = 0; u0 < NC / UNIT; u0 += BOTH) {
+        if (wcol + u0 * COLS >= ncols || !live) break;
+        if (lane == 0) ptx::tma_store_wait_read<C::STG_BUFS / 2 - 1>();   // these buffers' last stores have read them
         __syncwarp();
-        stage_row64(b, lane, words);
-        if (tma) {
-          ptx::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) ptx::tma_store_3d(&p.tm_d, ptx::smem_u32(b), c, drow, 0);
-        } else {
-          __syncwarp();
-          const long long pitch = p.ldd * (F32 ? 4 : 2);
-          copy_rows64<F32 ? 4 : 2>(b, lane, static_cast<char*>(p.D) + drow * pitch, pitch, rows, c, ncols, p.vec_d);
+        uint8_t* b = stg + stg_at * 4096;
+        stg_at = stg_at + 1 == C::STG_BUFS / 2 ? 0 : stg_at + 1;
+#pragma unroll
+        for (int u = u0; u < u0 + BOTH; ++u) {
+          float v[COLS];
+          const uint64_t* s = &sum[u * (UNIT / 2)];
+          if constexpr (!PAIR) {
+#pragma unroll
+            for (int i = 0; i < UNIT / 2; ++i) {
+              v[2 * i] = lo_of(s[i]);
+              v[2 * i + 1] = hi_of(s[i]);
+            }
+          } else if (p.pair == PAIR_SWIGLU) {      // the choice outside the loops: their elements interleave
+#pragma unroll
+            for (int i = 0; i < UNIT / 2; ++i) v[i] = silu_f(lo_of(s[i])) * hi_of(s[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < UNIT / 2; ++i) v[i] = gelu_f(lo_of(s[i])) * hi_of(s[i]);
+          }
+          uint32_t words[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) words[i] = F32 ? __float_as_uint(v[i]) : pack_bf16(v[2 * i % COLS], v[(2 * i + 1) % COLS]);
+          stage_row64(b + (u - u0) * 2048, lane, words);
+        }
+        if (tma) ptx::fence_proxy_async_smem();
+        __syncwarp();
+#pragma unroll
+        for (int u = u0; u < u0 + BOTH; ++u) {
+          const int c = wcol + u * COLS;
+          if (c >= ncols) break;
+          if (!tma) {
+            const long long pitch = p.ldd * (F32 ? 4 : 2);
+            copy_rows64<F32 ? 4 : 2>(b + (u - u0) * 2048, lane, static_cast<char*>(p.D) + drow * pitch, pitch, rows, c, ncols, p.vec_d);
+          } else if (lane == 0) {
+            ptx::tma_store_3d(&p.tm_d, ptx::smem_u32(b + (u - u0) * 2048), c, drow, 0);
+          }
         }
         if (lane == 0) ptx::tma_store_commit();
-        stg_at = stg_at + 1 == C::STG_BUFS ? 0 : stg_at + 1;
       }
       more = sched.next(p, *split, units, it);
       if (more) enter();

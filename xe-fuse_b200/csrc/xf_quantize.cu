@@ -434,7 +434,7 @@ static xf_status launch(const char* what, void (*fn)(Args...), unsigned grid, un
 }
 
 // Threads for a row: one chunk each where there are few rows, kAhead where other rows keep the SM busy
-// (4096 x 8192: 1024 threads of one chunk 76 us, 256 of four XX us).
+// (4096 x 8192: 1024 threads of one chunk 76 us, 256 of four 46 us).
 static unsigned row_threads(int M, int N) {
   const int chunks = (N + kChunk - 1) / kChunk, each = M >= 512 ? kAhead : 1;
   const int t = ((chunks + each - 1) / each + 31) / 32 * 32;

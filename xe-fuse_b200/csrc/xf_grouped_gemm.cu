@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -130,17 +131,20 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
   const Variant* v = nullptr;
   // The tile: the lower estimate of waves x clocks per tile.  A K block takes about 780 clocks on a pair's
   // 256 x 256 tile and 600 on a CTA's 128 x 128 tile with e4m3 (680 and 490 with bf16), the end of a tile 4500
-  // and 3000.  Pairs read half the operand bytes per multiplication; small tiles waste less on groups of few
-  // rows and spread better.  Rows of a group are taken to fill half of its last tile.
+  // and 3000, and sharing the tiles of the last wave 8000 and 5000.  Pairs read half the operand bytes per
+  // multiplication; small tiles waste less on groups of few rows and spread better.  Rows of a group are
+  // taken to fill half of its last tile.
   // Measured, pair against CTA: e4m3 4096 x 28672 x 4096 411 / 607 us, 777 x 5001 x 2000 37 / 27 us, bf16 with
   // 8 groups 4096 x 4096 x 4096 125 / 146 us.
   const int kblk = kind == KIND_BF16 ? 64 : 128;
   auto clocks = [&](int ctas) {
     const int side = 128 * ctas;
     const double tiles_m = d->num_groups == 1 ? (d->M + side - 1) / side : static_cast<double>(d->M) / side + 0.5 * d->num_groups;
-    const double waves = tiles_m * ((d->N + side - 1) / side) * ctas / sms;
+    const double waves = tiles_m * ((d->N + side - 1) / side) * ctas / sms, full = floor(waves);
     const double per_kb = kind == KIND_BF16 ? (ctas == 2 ? 680 : 490) : (ctas == 2 ? 780 : 600);
-    return (waves > 1 ? waves : 1) * ((d->K + kblk - 1) / kblk * per_kb + (ctas == 2 ? 4500 : 3000));
+    const double tile = (d->K + kblk - 1) / kblk * per_kb + (ctas == 2 ? 4500 : 3000);
+    const double last = waves == full ? 0.0 : (waves - full) * tile + (ctas == 2 ? 8000 : 5000);
+    return full * tile + (last < tile ? last : tile);
   };
   int ctas = clocks(2) < clocks(1) ? 2 : 1;
   if (d->flags & XF_FLAG_FORCE_1CTA) ctas = 1;
@@ -175,7 +179,7 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
       g->units = sms / v->ctas;
     }
   }
-  g->split_kb = d->flags & XF_FLAG_NO_SPLIT ? 0 : v->ctas == 2 ? 8 : 6;
+  g->split_kb = d->flags & XF_FLAG_NO_SPLIT ? 0 : v->ctas == 2 ? 10 : 8;
   if ((d->K + 63) / 64 > (1 << 20)) g->split_kb = 0;   // block numbers of a whole wave stay within 32 bits
   const size_t grid = static_cast<size_t>(g->units) * v->ctas;
   g->partials_off = 256 + (grid * 8 * sizeof(int) + 255) / 256 * 256;

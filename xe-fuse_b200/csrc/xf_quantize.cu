@@ -269,7 +269,7 @@ __device__ __forceinline__ void gated(const uint4& g, const uint4& u, float (&y)
   unpack(g, a);
   unpack(u, b);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = (GELU ? gelu_f(a[i]) : silu_f(a[i])) * b[i];
+  for (int i = 0; i < 8; ++i) y[i] = (GELU ? gelu_f(a[i]) : silu_fast(a[i])) * b[i];
 }
 
 // e4m3: 16 lanes per block of 128 columns, two blocks in flight; nothing is shared beyond the lanes.

@@ -436,7 +436,8 @@ typedef struct xf_grouped_gemm_desc {
   const float* scale_a; int64_t scale_a_row_stride, scale_a_blk_stride;          /* e4m3 only */
   const float* scale_b; int64_t scale_b_k_stride, scale_b_n_stride, scale_b_group_stride;
   void* D; int64_t ldd;          /* any alignment; 16-byte aligned rows are faster */
-  int32_t flags;                 /* XF_FLAG_FORCE_1CTA, _FORCE_2CTA, _NO_SPLIT, _NO_PDL, _SHORT_WAITS */
+  int32_t flags;                 /* XF_FLAG_FORCE_1CTA, _FORCE_2CTA, _FORCE_BN128, _FORCE_BN256, _NO_SPLIT,
+                                    _NO_PDL, _SHORT_WAITS */
   int32_t pad_;
   uint64_t workspace_bytes;      /* size of the workspace handed to xf_grouped_gemm_plan_create */
 } xf_grouped_gemm_desc;

@@ -92,6 +92,13 @@ def check(op, D, pair, before_D):
     assert torch.equal(D[:ends[0]], before_D[:ends[0]]) and torch.equal(D[ends[-1]:], before_D[ends[-1]:])
 
 
+def tiles(capi, dtype):
+    """Flags for: the planner's choice, then every tile, then the same without sharing the last wave's tiles."""
+    forced = [capi.FLAG_FORCE_1CTA | capi.FLAG_FORCE_BN128, capi.FLAG_FORCE_2CTA]
+    forced += [capi.FLAG_FORCE_1CTA | capi.FLAG_FORCE_BN256] if dtype == E4M3 else []
+    return [0] + forced + [f | capi.FLAG_NO_SPLIT for f in forced]
+
+
 def run(capi, op, dtype_d=torch.bfloat16, pair="none", flags=0, extra=0):
     M = op["A"].shape[0]
     N = op["B"].shape[-2 if op["b_nk"] else -1]
@@ -120,7 +127,7 @@ DENSE = [(1, 8, 16), (1, 1, 1), (3, 127, 127), (128, 128, 128), (129, 130, 129),
 @pytest.mark.parametrize("dtype", [E4M3, torch.bfloat16])
 def test_one_group(capi, cuda, M, N, K, nk, dtype):
     op = make(M, N, K, dtype=dtype, nk=nk)
-    for flags in (0, capi.FLAG_FORCE_1CTA | capi.FLAG_NO_SPLIT, capi.FLAG_FORCE_1CTA, capi.FLAG_FORCE_2CTA):
+    for flags in tiles(capi, dtype):
         run(capi, op, flags=flags)
     run(capi, op, torch.float32)
 
@@ -134,7 +141,7 @@ def test_outputs(capi, cuda, dtype_d, pair, extra, dtype):
     op = make(150, 390, 512, dtype=dtype)
     if dtype == torch.bfloat16:
         op["B"].mul_(512 ** -0.5)
-    for flags in (capi.FLAG_FORCE_1CTA, capi.FLAG_FORCE_2CTA):
+    for flags in tiles(capi, dtype)[1:4]:
         run(capi, op, dtype_d, pair, extra=extra, flags=flags)
 
 
@@ -150,7 +157,7 @@ def test_groups(capi, cuda, case, nk, dtype):
     sizes, M, before = GROUPS[case]
     N, K = (72, 80) if len(sizes) > 100 else (264, 700)
     op = make(M, N, K, sizes, dtype, nk, before)
-    for flags in (0, capi.FLAG_FORCE_1CTA | capi.FLAG_NO_SPLIT, capi.FLAG_FORCE_1CTA, capi.FLAG_FORCE_2CTA):
+    for flags in tiles(capi, dtype):
         run(capi, op, flags=flags)
     run(capi, op, torch.float32, pair="swiglu" if dtype == E4M3 else "none")
 
@@ -162,7 +169,7 @@ def test_long_sums_and_many_tiles(capi, cuda, dtype):
     for M, N, K, sizes in ((20, 300, 9000, None), (400, 300, 9000, None), (30, 200, 7000, [10, 0, 20]), (2100, 5200, 320, None),
                            (2600, 2000, 500, [900, 0, 1000, 3, 697])):
         op = make(M, N, K, sizes, dtype)
-        for flags in (0, capi.FLAG_FORCE_1CTA, capi.FLAG_FORCE_2CTA):
+        for flags in tiles(capi, dtype):
             _, first = run(capi, op, torch.float32, flags=flags)
             _, again = run(capi, op, torch.float32, flags=flags)
             assert torch.equal(first, again)     # fixed order of every sum

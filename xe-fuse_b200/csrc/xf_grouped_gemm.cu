@@ -42,7 +42,7 @@ static xf_status validate(const xf_grouped_gemm_desc* d) {
     set_error("%d groups need group_offsets", d->num_groups);
     return XF_ERR_INVALID_PROBLEM;
   }
-  if (d->flags & ~(XF_FLAG_FORCE_1CTA | XF_FLAG_FORCE_2CTA | XF_FLAG_NO_SPLIT | XF_FLAG_NO_PDL | XF_FLAG_SHORT_WAITS)) {
+  if (d->flags & ~(XF_FLAG_FORCE_1CTA | XF_FLAG_FORCE_2CTA | XF_FLAG_FORCE_BN128 | XF_FLAG_FORCE_BN256 | XF_FLAG_NO_SPLIT | XF_FLAG_NO_PDL | XF_FLAG_SHORT_WAITS)) {
     set_error("unsupported flags 0x%x", d->flags);
     return XF_ERR_NOT_SUPPORTED;
   }
@@ -128,30 +128,37 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
     return XF_ERR_ARCH_MISMATCH;
   }
   const int kind = d->dtype_ab == XF_DT_BF16 ? KIND_BF16 : KIND_E4M3;
+  // The tile: the lowest estimate of waves x clocks per tile.  Measured on long problems: a K block, the end of
+  // a tile and the sharing of the last wave's tiles take about
+  //   e4m3  256 x 256, CTA pair  720 + 3700 + 8000     bf16  256 x 256, CTA pair  680 + 3700 + 8000
+  //         128 x 256, one CTA   870 + 3700 + 8000           128 x 128, one CTA   490 + 2000 + 5000
+  //         128 x 128, one CTA   600 + 2000 + 5000
+  // clocks.  Large tiles read fewer operand bytes per multiplication; tiles of 128 rows waste less on groups
+  // of few rows, and small ones spread better.  Rows of a group are taken to fill half of its last tile.
   const Variant* v = nullptr;
-  // The tile: the lower estimate of waves x clocks per tile.  A K block takes about 780 clocks on a pair's
-  // 256 x 256 tile and 600 on a CTA's 128 x 128 tile with e4m3 (680 and 490 with bf16), the end of a tile 4500
-  // and 3000, and sharing the tiles of the last wave 8000 and 5000.  Pairs read half the operand bytes per
-  // multiplication; small tiles waste less on groups of few rows and spread better.  Rows of a group are
-  // taken to fill half of its last tile.
-  // Measured, pair against CTA: e4m3 4096 x 28672 x 4096 411 / 607 us, 777 x 5001 x 2000 37 / 27 us, bf16 with
-  // 8 groups 4096 x 4096 x 4096 125 / 146 us.
-  const int kblk = kind == KIND_BF16 ? 64 : 128;
-  auto clocks = [&](int ctas) {
-    const int side = 128 * ctas;
-    const double tiles_m = d->num_groups == 1 ? (d->M + side - 1) / side : static_cast<double>(d->M) / side + 0.5 * d->num_groups;
-    const double waves = tiles_m * ((d->N + side - 1) / side) * ctas / sms, full = floor(waves);
-    const double per_kb = kind == KIND_BF16 ? (ctas == 2 ? 680 : 490) : (ctas == 2 ? 780 : 600);
-    const double tile = (d->K + kblk - 1) / kblk * per_kb + (ctas == 2 ? 4500 : 3000);
-    const double last = waves == full ? 0.0 : (waves - full) * tile + (ctas == 2 ? 8000 : 5000);
-    return full * tile + (last < tile ? last : tile);
-  };
-  int ctas = clocks(2) < clocks(1) ? 2 : 1;
-  if (d->flags & XF_FLAG_FORCE_1CTA) ctas = 1;
-  else if (d->flags & XF_FLAG_FORCE_2CTA) ctas = 2;
-  for (int i = 0; i < kTilesPerKind; ++i) {
-    const Variant& c = kind == KIND_BF16 ? g_variants_bf16[i] : g_variants_e4m3[i];
-    if (c.ctas == ctas) v = &c;
+  const Variant* all = kind == KIND_BF16 ? g_variants_bf16 : g_variants_e4m3;
+  const int count = kind == KIND_BF16 ? kTilesBf16 : kTilesE4m3, kblk = kind == KIND_BF16 ? 64 : 128;
+  double best = 0.0;
+  for (int i = 0; i < count; ++i) {
+    const Variant& c = all[i];
+    if ((d->flags & XF_FLAG_FORCE_1CTA && c.ctas != 1) || (d->flags & XF_FLAG_FORCE_2CTA && c.ctas != 2) ||
+        (d->flags & XF_FLAG_FORCE_BN128 && c.bn != 128) || (d->flags & XF_FLAG_FORCE_BN256 && c.bn != 256))
+      continue;
+    const int rows = 128 * c.ctas;
+    const double tiles_m = d->num_groups == 1 ? (d->M + rows - 1) / rows : static_cast<double>(d->M) / rows + 0.5 * d->num_groups;
+    const double waves = tiles_m * ((d->N + c.bn - 1) / c.bn) * c.ctas / sms, full = floor(waves);
+    const double per_kb = kind == KIND_BF16 ? (c.bn == 256 ? 680 : 490) : (c.ctas == 2 ? 720 : c.bn == 256 ? 870 : 600);
+    const double tile = (d->K + kblk - 1) / kblk * per_kb + (c.bn == 256 ? 3700 : 2000);
+    const double last = waves == full ? 0.0 : (waves - full) * tile + (c.bn == 256 ? 8000 : 5000);
+    const double cost = full * tile + (last < tile ? last : tile);
+    if (!v || cost < best) {
+      v = &c;
+      best = cost;
+    }
+  }
+  if (!v) {
+    set_error("no tile of this type matches the flags 0x%x", d->flags);
+    return XF_ERR_NOT_SUPPORTED;
   }
   const bool f32 = d->dtype_d == XF_DT_F32;
   g->fn = v->fn[d->pair == XF_PAIR_NONE ? (f32 ? OUT_F32 : OUT_BF16) : (f32 ? OUT_PAIR_F32 : OUT_PAIR_BF16)];
@@ -179,7 +186,7 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
       g->units = sms / v->ctas;
     }
   }
-  g->split_kb = d->flags & XF_FLAG_NO_SPLIT ? 0 : v->ctas == 2 ? 10 : 8;
+  g->split_kb = d->flags & XF_FLAG_NO_SPLIT ? 0 : v->bn == 256 ? 10 : 8;   // 8000 and 5000 clocks
   if ((d->K + 63) / 64 > (1 << 20)) g->split_kb = 0;   // block numbers of a whole wave stay within 32 bits
   const size_t grid = static_cast<size_t>(g->units) * v->ctas;
   g->partials_off = 256 + (grid * 8 * sizeof(int) + 255) / 256 * 256;

@@ -4,7 +4,7 @@
 namespace xf {
 namespace grouped {
 
-const Variant g_variants_bf16[kTilesPerKind] = {
+const Variant g_variants_bf16[kTilesBf16] = {
     XF_GROUPED_VARIANT(KIND_BF16, 256, 2, "bf16_256x256_cta2"),
     XF_GROUPED_VARIANT(KIND_BF16, 128, 1, "bf16_128x128_cta1"),
 };

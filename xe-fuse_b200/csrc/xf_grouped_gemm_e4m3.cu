@@ -4,8 +4,9 @@
 namespace xf {
 namespace grouped {
 
-const Variant g_variants_e4m3[kTilesPerKind] = {
+const Variant g_variants_e4m3[kTilesE4m3] = {
     XF_GROUPED_VARIANT(KIND_E4M3, 256, 2, "e4m3_256x256_cta2"),
+    XF_GROUPED_VARIANT(KIND_E4M3, 256, 1, "e4m3_128x256_cta1"),
     XF_GROUPED_VARIANT(KIND_E4M3, 128, 1, "e4m3_128x128_cta1"),
 };
 

@@ -74,17 +74,17 @@ struct Cfg {
   static constexpr int A_BYTES = 128 * 128;
   static constexpr int B_BYTES = BN_CTA * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = CTAS == 2 ? 4 : 5;
+  static constexpr int STAGES = CTAS == 2 ? 4 : BN == 256 ? 3 : 5;
   static constexpr int NBUF = 512 / BN;                 // accumulators in TMEM
   static constexpr int NC = BN / 2;                     // columns per epilogue warp
   static constexpr bool SPLIT_REGS = NC == 128;
-  static constexpr int STG_BUFS = CTAS == 2 ? 4 : 2;    // staging buffers per epilogue warp: 32 rows x 64 bytes
+  static constexpr int STG_BUFS = NC / 32;        // staging buffers per epilogue warp: 32 rows x 64 bytes
   static constexpr int STG_BYTES = STG_BUFS * 2048;
   static constexpr int BAR_BYTES = 256;
   static constexpr int TAB_BYTES = (kMaxGroups + 1 + 2 * kMaxGroups) * 4;   // first tile, {first row, rows} of a group
   static constexpr int LIST_BYTES = kTileList * 16;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 8 * STG_BYTES + BAR_BYTES + LIST_BYTES + TAB_BYTES;
-  static_assert(BN_CTA == 128, "a CTA loads 128 columns of B");
+  static_assert(BN_CTA % 128 == 0, "B is loaded in boxes of 128 columns");
   static_assert(NC % 64 == 0 && NC <= 128, "an epilogue warp's columns share one scale of B");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 };
@@ -380,7 +380,9 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
             for (int b = 0; b < boxes; ++b) ptx::tma_load_3d<CTAS>(sa + b * 4096, &p.tm_a32, bar, k, row + b * 32, 0);
           }
           if (p.b_nk) {
-            ptx::tma_load_3d<CTAS>(sb, &p.tm_b, bar, k, col, bg);
+#pragma unroll
+            for (int c = 0; c < C::BN_CTA / 128; ++c)
+              ptx::tma_load_3d<CTAS>(sb + c * 16384, &p.tm_b, bar, k, col + c * 128, bg);
           } else {
 #pragma unroll
             for (int c = 0; c < C::BN_CTA / C::GRP_COLS; ++c)
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
     const uint32_t t_base = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * NC);
     const int ncols = OUT == OUT_PAIR_BF16 || OUT == OUT_PAIR_F32 ? p.N >> 1 : p.N;
     const uint32_t tfull0 = ptx::smem_u32(tfull_bar);
-    int buf = 0, stg_at = 0;
+    int buf = 0;
     uint32_t tphase = 0;
     // A tile as this warp sees it: its place, and where its block scales are (the first two on their way).
     // (Entering the next tile before the results of the last one have left costs registers that the loop over
@@ -579,21 +581,20 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         if (lane < count) *reinterpret_cast<volatile int*>(flag) = 0;   // for the next launch
       }
       const int wcol = OUT == OUT_PAIR_BF16 || OUT == OUT_PAIR_F32 ? col >> 1 : col, drow = x.row0 + roff;
-      // 64 bytes of each row make a unit; two of them are staged before one fence hands them to the store engine
+      // 64 bytes of each row make a unit; as many as there are buffers are staged before one fence hands them to
+      // the store engine
       constexpr bool F32 = OUT == OUT_F32 || OUT == OUT_PAIR_F32, PAIR = OUT == OUT_PAIR_BF16 || OUT == OUT_PAIR_F32;
       constexpr int UNIT = (F32 ? 16 : 32) * (PAIR ? 2 : 1);     // sums that make 64 bytes of D
       constexpr int COLS = F32 ? 16 : 32;
-      constexpr int BOTH = NC / UNIT > 1 ? 2 : 1;
+      constexpr int ROUND = NC / UNIT < C::STG_BUFS ? NC / UNIT : C::STG_BUFS;
       const bool tma = p.vec_d && rows >= 32;    // a tensor map's box has 32 rows, all of this group
 #pragma unroll
-      for (int u0 = 0; u0 < NC / UNIT; u0 += BOTH) {
+      for (int u0 = 0; u0 < NC / UNIT; u0 += ROUND) {
         if (wcol + u0 * COLS >= ncols || !live) break;
-        if (lane == 0) ptx::tma_store_wait_read<C::STG_BUFS / 2 - 1>();   // these buffers' last stores have read them
+        if (lane == 0) ptx::tma_store_wait_read<0>();   // the last round's stores have read the buffers
         __syncwarp();
-        uint8_t* b = stg + stg_at * 4096;
-        stg_at = stg_at + 1 == C::STG_BUFS / 2 ? 0 : stg_at + 1;
 #pragma unroll
-        for (int u = u0; u < u0 + BOTH; ++u) {
+        for (int u = u0; u < u0 + ROUND; ++u) {
           float v[COLS];
           const uint64_t* s = &sum[u * (UNIT / 2)];
           if constexpr (!PAIR) {
@@ -612,19 +613,19 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
           uint32_t words[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) words[i] = F32 ? __float_as_uint(v[i]) : pack_bf16(v[2 * i % COLS], v[(2 * i + 1) % COLS]);
-          stage_row64(b + (u - u0) * 2048, lane, words);
+          stage_row64(stg + (u - u0) * 2048, lane, words);
         }
         if (tma) ptx::fence_proxy_async_smem();
         __syncwarp();
 #pragma unroll
-        for (int u = u0; u < u0 + BOTH; ++u) {
+        for (int u = u0; u < u0 + ROUND; ++u) {
           const int c = wcol + u * COLS;
           if (c >= ncols) break;
           if (!tma) {
             const long long pitch = p.ldd * (F32 ? 4 : 2);
-            copy_rows64<F32 ? 4 : 2>(b + (u - u0) * 2048, lane, static_cast<char*>(p.D) + drow * pitch, pitch, rows, c, ncols, p.vec_d);
+            copy_rows64<F32 ? 4 : 2>(stg + (u - u0) * 2048, lane, static_cast<char*>(p.D) + drow * pitch, pitch, rows, c, ncols, p.vec_d);
           } else if (lane == 0) {
-            ptx::tma_store_3d(&p.tm_d, ptx::smem_u32(b + (u - u0) * 2048), c, drow, 0);
+            ptx::tma_store_3d(&p.tm_d, ptx::smem_u32(stg + (u - u0) * 2048), c, drow, 0);
           }
         }
         if (lane == 0) ptx::tma_store_commit();
@@ -663,8 +664,8 @@ struct Variant {
    {grouped_gemm_kernel<KIND, BN, CTAS, OUT_BF16>, grouped_gemm_kernel<KIND, BN, CTAS, OUT_PAIR_BF16>,   \
     grouped_gemm_kernel<KIND, BN, CTAS, OUT_F32>, grouped_gemm_kernel<KIND, BN, CTAS, OUT_PAIR_F32>},    \
    NAME}
-static const int kTilesPerKind = 2;
-extern const Variant g_variants_bf16[kTilesPerKind], g_variants_e4m3[kTilesPerKind];
+static const int kTilesBf16 = 2, kTilesE4m3 = 3;
+extern const Variant g_variants_bf16[kTilesBf16], g_variants_e4m3[kTilesE4m3];
 
 }  // namespace grouped
 }  // namespace xf

@@ -111,7 +111,7 @@ struct Geometry {
   const Variant* v;
   KernelFn fn;
   int dev, units;
-  int split_kb;            // 0: whole tiles only
+  int split_kb, split_max;   // Params; split_kb 0: whole tiles only
   size_t partials_off, workspace_bytes;   // [0, 256) status, flags, partial sums
 };
 
@@ -128,32 +128,43 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
     return XF_ERR_ARCH_MISMATCH;
   }
   const int kind = d->dtype_ab == XF_DT_BF16 ? KIND_BF16 : KIND_E4M3;
-  // The tile: the lowest estimate of waves x clocks per tile.  Measured on long problems: a K block, the end of
-  // a tile and the sharing of the last wave's tiles take about
-  //   e4m3  256 x 256, CTA pair  720 + 3700 + 8000     bf16  256 x 256, CTA pair  680 + 3700 + 8000
-  //         128 x 256, one CTA   870 + 3700 + 8000           128 x 128, one CTA   490 + 2000 + 5000
-  //         128 x 128, one CTA   600 + 2000 + 5000
-  // clocks.  Large tiles read fewer operand bytes per multiplication; tiles of 128 rows waste less on groups
-  // of few rows, and small ones spread better.  Rows of a group are taken to fill half of its last tile.
+  // The tile: the lowest estimate of clocks for whole waves plus the last one, whose tiles may be shared.
+  // Measured on long problems, in clocks for a K block, the end of a tile, publishing a share of one and
+  // summing another unit's share:
+  //   e4m3  256 x 256, CTA pair  720  3700  5000  1800     bf16  256 x 256, CTA pair  680  3700  5000  1800
+  //         128 x 256, one CTA   870  3700  5000  1800           128 x 128, one CTA   490  2000  3000   900
+  //         128 x 128, one CTA   600  2000  3000   900
+  // Large tiles read fewer operand bytes per multiplication; tiles of 128 rows waste less on groups of few
+  // rows, and small ones spread better.  Rows of a group are taken to fill half of its last tile.  e4m3, pair /
+  // 128 x 256 / 128 x 128: 4096 x 28672 x 4096 402 / 446 / 530 us, 777 x 5001 x 2000 34 / 20 / 24 us,
+  // 64 experts 16384 x 4096 x 2048 262 / 215 / 236 us, 100 x 8192 x 8192 - / 23 / 16.5 us.
   const Variant* v = nullptr;
   const Variant* all = kind == KIND_BF16 ? g_variants_bf16 : g_variants_e4m3;
   const int count = kind == KIND_BF16 ? kTilesBf16 : kTilesE4m3, kblk = kind == KIND_BF16 ? 64 : 128;
+  const double num_kb = (d->K + kblk - 1) / kblk;
   double best = 0.0;
   for (int i = 0; i < count; ++i) {
     const Variant& c = all[i];
     if ((d->flags & XF_FLAG_FORCE_1CTA && c.ctas != 1) || (d->flags & XF_FLAG_FORCE_2CTA && c.ctas != 2) ||
         (d->flags & XF_FLAG_FORCE_BN128 && c.bn != 128) || (d->flags & XF_FLAG_FORCE_BN256 && c.bn != 256))
       continue;
-    const int rows = 128 * c.ctas;
+    const bool wide = c.bn == 256;
+    const double per_kb = kind == KIND_BF16 ? (wide ? 680 : 490) : (c.ctas == 2 ? 720 : wide ? 870 : 600);
+    const double tile = num_kb * per_kb + (wide ? 3700 : 2000), publish = wide ? 5000 : 3000, sum = wide ? 1800 : 900;
+    const int rows = 128 * c.ctas, units = sms / c.ctas;
+    // sharing a tile's K range s ways takes tile / s + publish + (s - 1) * sum: least at s = sqrt(tile / sum)
+    const int most = static_cast<int>(sqrt(num_kb * per_kb / sum) + 0.5);
+    const int split_max = most < 2 ? 2 : most > 8 ? 8 : most;
     const double tiles_m = d->num_groups == 1 ? (d->M + rows - 1) / rows : static_cast<double>(d->M) / rows + 0.5 * d->num_groups;
-    const double waves = tiles_m * ((d->N + c.bn - 1) / c.bn) * c.ctas / sms, full = floor(waves);
-    const double per_kb = kind == KIND_BF16 ? (c.bn == 256 ? 680 : 490) : (c.ctas == 2 ? 720 : c.bn == 256 ? 870 : 600);
-    const double tile = (d->K + kblk - 1) / kblk * per_kb + (c.bn == 256 ? 3700 : 2000);
-    const double last = waves == full ? 0.0 : (waves - full) * tile + (c.bn == 256 ? 8000 : 5000);
-    const double cost = full * tile + (last < tile ? last : tile);
+    const double waves = tiles_m * ((d->N + c.bn - 1) / c.bn) / units, full = floor(waves), rest = waves - full;
+    const double share = rest * split_max < 1.0 ? 1.0 / split_max : rest;
+    const double last = rest == 0.0 ? 0.0 : share * tile + publish + (1.0 / share < 2.0 ? 1.0 : 1.0 / share - 1.0) * sum;
+    const double cost = full * tile + (last < tile || rest == 0.0 ? last : tile);
     if (!v || cost < best) {
       v = &c;
       best = cost;
+      g->split_kb = static_cast<int>((publish + sum) / per_kb + 0.5);
+      g->split_max = split_max;
     }
   }
   if (!v) {
@@ -186,7 +197,7 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
       g->units = sms / v->ctas;
     }
   }
-  g->split_kb = d->flags & XF_FLAG_NO_SPLIT ? 0 : v->bn == 256 ? 10 : 8;   // 8000 and 5000 clocks
+  if (d->flags & XF_FLAG_NO_SPLIT) g->split_kb = 0;
   if ((d->K + 63) / 64 > (1 << 20)) g->split_kb = 0;   // block numbers of a whole wave stay within 32 bits
   const size_t grid = static_cast<size_t>(g->units) * v->ctas;
   g->partials_off = 256 + (grid * 8 * sizeof(int) + 255) / 256 * 256;
@@ -305,6 +316,7 @@ xf_status xf_grouped_gemm_plan_create(const xf_grouped_gemm_desc* d, void* works
     plan->clear_bytes = 256;
     if (g.split_kb && d->workspace_bytes >= g.workspace_bytes) {
       p.split_kb = g.split_kb;
+      p.split_max = g.split_max;
       p.flags = reinterpret_cast<int*>(static_cast<char*>(workspace) + 256);
       p.partials = reinterpret_cast<float4*>(static_cast<char*>(workspace) + g.partials_off);
       plan->clear_bytes = g.partials_off;

@@ -56,7 +56,8 @@ struct alignas(64) Params {
   long long wait_budget;
   // Tiles whose K range several units share (split_kb > 0: see Split): one flag per epilogue warp and one
   // slot of partial sums per CTA.
-  int split_kb;          // what sharing costs, in K blocks of one unit
+  int split_kb;          // what sharing a tile between two units costs, in K blocks of one unit
+  int split_max;         // most units that share a tile: they are summed one by one
   int* flags;            // [grid][8], zero between launches
   float4* partials;      // [grid][8 warps][columns of a warp / 4][32 lanes]
 };
@@ -142,9 +143,9 @@ struct Split {
     whole = tiles;
     sharers = lo = hi = 0;
     if (p.split_kb == 0 || rest == 0) return;
-    // At least 4 blocks for each unit, at most 8 units for each tile (they are summed one by one), and where
-    // two or more units go to a tile the same number to each: a range that touches two tiles adds a sharer.
-    int n = min(min(units, 8 * rest), rest * p.num_kb / 4);
+    // At least 4 blocks for each unit, and where two or more units go to a tile the same number to each: a
+    // range that touches two tiles adds a sharer.
+    int n = min(min(units, p.split_max * rest), rest * p.num_kb / 4);
     if (n >= 2 * rest) n -= n % rest;
     if (n <= rest || (n - rest) * static_cast<long long>(p.num_kb) <= static_cast<long long>(p.split_kb) * n) return;
     sharers = n;

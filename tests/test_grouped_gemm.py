@@ -315,6 +315,27 @@ def test_feed_forward_in_8_bits(capi, cuda, experts):
             assert float((y[lo:hi].double() - full).norm() / full.norm()) < 3 * 2.0 ** -4
 
 
+@pytest.mark.gpu
+def test_offsets_past_32_bits(capi, cuda):
+    """Rows of A and D that start beyond 4 GB, and weights of a group beyond it."""
+    M, N, K, pitch = 70000, 64, 96, 65536
+    op = make(40, N, K, [40])
+    A = torch.empty(M, pitch, device=cuda, dtype=torch.int8).view(E4M3)[:, :K]
+    A[-40:].view(torch.int8).copy_(op["A"].view(torch.int8))
+    B = torch.empty(1 << 33, device=cuda, dtype=torch.int8).view(E4M3).as_strided((3, K, N), ((1 << 32) - 4096 * 16, N, 1))
+    B[2].view(torch.int8).copy_(op["B"][0].view(torch.int8))
+    sa = torch.ones(M, 1, device=cuda)
+    sa[-40:] = op["scale_a"]
+    sb = op["scale_b"].expand(3, -1, -1)
+    D = torch.empty(M, pitch // 2, device=cuda, dtype=torch.bfloat16)[:, :N]
+    off = torch.tensor([M - 40, M - 40, M - 40, M], dtype=torch.int32, device=cuda)
+    for flags in tiles(capi, E4M3):
+        D[-40:] = 0
+        capi.GroupedGemmPlan(A, B, D, offsets=off, scale_a=sa, scale_b=sb, flags=flags).run()
+        torch.cuda.synchronize()
+        check(op, D[-40:].contiguous(), "none", D[-40:])
+
+
 # ------------------------------------------------------------------ refusals: no GPU is touched
 def desc(capi, **k):
     d = capi.XfGroupedGemmDesc()

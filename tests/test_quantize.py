@@ -204,6 +204,26 @@ def test_no_rows_and_other_streams(capi, cuda):
     assert torch.equal(q.view(torch.int8), want_q.view(torch.int8)) and torch.equal(scale, want_s)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("s8", [False, True])
+def test_offsets_past_32_bits(capi, cuda, s8):
+    M, N, pitch = 40000, 256, 65536                  # the last rows start beyond 2^31 elements
+    x = torch.empty(M, pitch, device=cuda, dtype=torch.bfloat16)[:, :N]
+    x[:, :] = torch.randn(1, N, device=cuda)
+    x[-3:] = torch.randn(3, N, device=cuda).to(torch.bfloat16)
+    q = torch.empty(M, pitch * 2, device=cuda, dtype=torch.int8)[:, :N]
+    q = q if s8 else q.view(E4M3)
+    scale = torch.empty(M, device=cuda) if s8 else torch.empty(2, M, device=cuda).t()
+    capi.rms_norm_quantize(q, scale, x, None, eps=1e-5)
+    torch.cuda.synchronize()
+    check_norm(x[-3:], None, q[-3:], scale[-3:], s8, 1e-5, 8)
+    half = N // 2
+    sc = torch.empty(M, device=cuda) if s8 else torch.empty(1, M, device=cuda).t()
+    capi.act_mul_quantize(q[:, :half], sc, x)
+    torch.cuda.synchronize()
+    check_act(x[-3:], half, q[-3:, :half], sc[-3:], s8, False)
+
+
 # ------------------------------------------------------------------ refusals: no GPU is touched
 def desc(capi, **k):
     """A packed xf_quantize_desc of a valid norm, with some fields changed."""

@@ -368,8 +368,8 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       const int bg = p.b_grouped ? x.g : 0;
       for (int kb = it.kb0; kb < it.kb1; ++kb) {
         w.wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, DEV_TIMEOUT_PRODUCER_EMPTY);
-        __syncwarp();
-        if (ptx::elect_one()) {
+        // once a wait has run out nothing more is loaded: a stage's barrier may still be in its last phase
+        if (!w.any_lost() && ptx::elect_one()) {
           const uint32_t own = ptx::smem_u32(&full_bar[stage]);
           const uint32_t bar = CTAS == 2 ? ptx::mapa(own, 0) : own;
           if (rank == 0) ptx::mbar_arrive_expect_tx(own, bytes);
@@ -426,9 +426,9 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
           const uint32_t d = tmem + static_cast<uint32_t>(buf * BN);
           // last of all, the wait that the promotion warps answer: what follows it is on their round trip
           if (fresh) w.wait(tempty0 + buf * 8, tphase ^ 1u, DEV_TIMEOUT_MMA_TMEM_EMPTY);
-          __syncwarp();
+          const bool lost = w.any_lost();
           ptx::tc_fence_after();
-          if (ptx::elect_one()) {
+          if (!lost && ptx::elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               ptx::umma<KIND, CTAS>(d, adesc + static_cast<uint64_t>(2 * k), bdesc + k * b_step, idesc,

@@ -184,6 +184,7 @@ struct Waiter {
       lost = true;
     }
   }
+  __device__ __forceinline__ bool any_lost() const { return __any_sync(0xffffffffu, lost); }
   // Until other CTAs have set the flags that the lanes name; by a converged warp (a loop in one lane only
   // made the compiler spill what lives in registers around it).
   __device__ __forceinline__ void wait_flags(const int* flag, int code) {

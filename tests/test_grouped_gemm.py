@@ -375,7 +375,7 @@ def test_null_arguments(capi):
 
 
 def test_wrapper_refusals(capi, monkeypatch):
-    monkeypatch.setattr(capi, "_on_current_device", lambda *t: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)       # what a CPU tensor reports
     A, B, D = torch.zeros(8, 256, dtype=E4M3), torch.zeros(256, 128, dtype=E4M3), torch.zeros(8, 128)
     sa, sb, off = torch.ones(8, 2), torch.ones(2, 1), torch.zeros(3, dtype=torch.int32)
     for a, k in (

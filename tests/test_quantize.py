@@ -89,7 +89,7 @@ def test_norm(capi, cuda, M, N, residual, s8, extra):
         hout = torch.zeros(M, N, device=cuda, dtype=torch.bfloat16) if residual == "apart" else None
     capi.rms_norm_quantize(q, scale, x, w, res, hout, 1e-5)
     torch.cuda.synchronize()
-    terms = 8 * math.ceil(N / 8 / 1024)
+    terms = 16 * math.ceil(N / 16 / 512)      # 512 threads at most, 16 columns at a time
     check_norm(h, w, q, scale, s8, 1e-5, terms)
     assert bool((whole[:, N:] == 77).all())
     if residual:
@@ -115,7 +115,7 @@ def test_norm_special_rows(capi, cuda, s8):
     v = q.double() * (scale.double()[:, None] if s8 else scale.double().repeat_interleave(128, 1))
     assert bool((q[0].float() == 0).all()) and bool(torch.isfinite(scale[0]).all()) and bool((scale[0] > 0).all())
     assert bool((q[1, 128:256].float() == 0).all())
-    check_norm(x[1:2], None, q[1:2], scale[1:2], s8, 1e-6, 8)
+    check_norm(x[1:2], None, q[1:2], scale[1:2], s8, 1e-6, 16)
     assert bool(torch.isnan(scale[2]).all())   # the row's mean is NaN
     assert bool(torch.isnan(scale[3]).any())   # inf * rstd, rstd = 0
     assert bool(torch.isfinite(v[4]).all()) and bool((v[4].abs() <= 1.001e-35).all())
@@ -216,7 +216,7 @@ def test_offsets_past_32_bits(capi, cuda, s8):
     scale = torch.empty(M, device=cuda) if s8 else torch.empty(2, M, device=cuda).t()
     capi.rms_norm_quantize(q, scale, x, None, eps=1e-5)
     torch.cuda.synchronize()
-    check_norm(x[-3:], None, q[-3:], scale[-3:], s8, 1e-5, 8)
+    check_norm(x[-3:], None, q[-3:], scale[-3:], s8, 1e-5, 16)
     half = N // 2
     sc = torch.empty(M, device=cuda) if s8 else torch.empty(1, M, device=cuda).t()
     capi.act_mul_quantize(q[:, :half], sc, x)
@@ -275,7 +275,7 @@ def test_empty_calls(capi):
 
 
 def test_wrapper_refusals(capi, monkeypatch):
-    monkeypatch.setattr(capi, "_on_current_device", lambda *t: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)       # what a CPU tensor reports
     x, s = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(4, 2)
     q = torch.zeros(4, 256, dtype=E4M3)
     for bad in (

@@ -299,15 +299,18 @@ class GroupedGemmPlan:
         L_ = lib()
         self.handle = C.c_void_p()
         self._keep = [A, B, D, offsets, scale_a, scale_b]
-        _on_current_device(*self._keep)
+        device = torch.cuda.current_device()
+        for t in self._keep:
+            if t is not None and t.get_device() != device:
+                raise XfError(4, f"tensor on {t.device}, but the current device is cuda:{device}")
         if B.dtype != A.dtype:
             raise XfError(2, f"A and B must have one type, got {A.dtype} and {B.dtype}")
         M, K = A.shape
         N = B.shape[-2] if b_nk else B.shape[-1]
         G = offsets.shape[0] - 1 if offsets is not None else 1
         lead = () if B.dim() == 2 else (G,)
-        lda = _rows(A, "A", (M, K), A.dtype)
-        ldd = _rows(D, "D", (M, N if pair == "none" else N // 2), D.dtype)
+        lda = _rows(A, "A", (M, K), A.dtype, device)
+        ldd = _rows(D, "D", (M, N if pair == "none" else N // 2), D.dtype, device)
         if tuple(B.shape) != lead + ((N, K) if b_nk else (K, N)) or (B.shape[-1] > 1 and B.stride(-1) != 1):
             raise XfError(3, f"B: {tuple(B.shape)} with strides {B.stride()} does not fit A {tuple(A.shape)} and {G} groups")
         if offsets is not None and (offsets.dtype != torch.int32 or offsets.dim() != 1 or not offsets.is_contiguous()):
@@ -502,42 +505,36 @@ def ve_dequant_rotary(out, acc, scale_token, scale_channel, cos_sin):
 _QUANTIZE_DESC = struct.Struct("=6Q6q3ifii")
 
 
-def _rows(t, what, shape, dtype):
-    """Checks a matrix with contiguous columns and returns its row pitch."""
+def _rows(t, what, shape, dtype, device):
+    """Checks a matrix with contiguous columns on the current device and returns its row pitch."""
+    st = t.stride()
     if t.dtype != dtype:
         raise XfError(2, f"{what}: expected {dtype}, got {t.dtype}")
-    st = t.stride()
     if t.shape != shape or (st[1] != 1 and shape[1] > 1):
         raise XfError(3, f"{what}: expected a {tuple(shape)} tensor with contiguous columns, got "
                          f"{tuple(t.shape)} with strides {st}")
+    if t.get_device() != device:
+        raise XfError(4, f"{what}: on {t.device}, but the current device is {device}")
     return st[0] if shape[0] > 1 else -(-shape[1] // 16) * 16    # a single row's pitch is of no use
 
 
-def _on_current_device(*tensors):
+def _codes(out, scale, shape, device):
+    """(type, row pitch, row stride and block stride of the scales) of an 8-bit output."""
     import torch
-    cur = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != cur:
-            raise XfError(4, f"tensor on {t.device}, but cuda:{cur} is the current device")
-
-
-def _codes(out, scale):
-    """(output type, row stride, block stride of the scales) of an 8-bit [M, N] output."""
-    import torch
-    M, N = out.shape
-    st = scale.stride()
-    if scale.dtype != torch.float32:
-        raise XfError(2, f"scale: expected float32, got {scale.dtype}")
-    if out.dtype == torch.float8_e4m3fn:
-        if scale.shape != (M, -(-N // 128)):
-            raise XfError(3, f"scale: expected {(M, -(-N // 128))}, got {tuple(scale.shape)}")
-        # a dimension of one has no meaningful stride
-        return DT_E4M3, st[0] if M > 1 else 1, st[1] if N > 128 else 1
-    if out.dtype != torch.int8:
-        raise XfError(2, f"out: int8 or float8_e4m3fn, got {out.dtype}")
-    if scale.shape != (M,):
-        raise XfError(3, f"scale: expected {(M,)}, got {tuple(scale.shape)}")
-    return DT_S8, st[0] if M > 1 else 1, 1
+    dtype, (M, N), st = out.dtype, shape, scale.stride()
+    if dtype == torch.float8_e4m3fn:
+        code, want = DT_E4M3, (M, -(-N // 128))
+    elif dtype == torch.int8:
+        code, want = DT_S8, (M,)
+    else:
+        raise XfError(2, f"out: int8 or float8_e4m3fn, got {dtype}")
+    if scale.dtype != torch.float32 or scale.shape != want:
+        raise XfError(3, f"scale: expected float32 {want}, got {scale.dtype} {tuple(scale.shape)}")
+    if scale.get_device() != device:
+        raise XfError(4, f"scale: on {scale.device}, but the current device is {device}")
+    # a dimension of one has no meaningful stride
+    return (code, _rows(out, "out", shape, dtype, device), st[0] if M > 1 else 1,
+            st[1] if N > 128 and code == DT_E4M3 else 1)
 
 
 def rms_norm_quantize(out, scale, inp, weight=None, residual=None, residual_out=None, eps=1e-6):
@@ -545,23 +542,24 @@ def rms_norm_quantize(out, scale, inp, weight=None, residual=None, residual_out=
     place when that is None).  out int8 with scale [M], or float8_e4m3fn with scale [M, ceil(N/128)] of any
     strides (the block-scaled products read fastest with the rows side by side: torch.empty(blocks, M).t())."""
     import torch
-    shape, bf16 = inp.shape, torch.bfloat16
+    shape, bf16, device = inp.shape, torch.bfloat16, torch.cuda.current_device()
     M, N = shape
-    _on_current_device(out, scale, inp, weight, residual, residual_out)
-    code, sr, sb = _codes(out, scale)
-    il, ol = _rows(inp, "inp", shape, bf16), _rows(out, "out", shape, out.dtype)
-    rp = hp = rl = hl = 0
+    code, ol, sr, sb = _codes(out, scale, shape, device)
+    il = _rows(inp, "inp", shape, bf16, device)
+    rp = hp = rl = hl = wp = 0
     if residual is not None:
         if residual_out is None:
             residual_out = residual
-        rp, rl = residual.data_ptr(), _rows(residual, "residual", shape, bf16)
-        hp, hl = residual_out.data_ptr(), _rows(residual_out, "residual_out", shape, bf16)
-    if weight is not None and (weight.dtype != bf16 or weight.shape != (N,) or not weight.is_contiguous()):
-        raise XfError(3, f"weight: expected contiguous bfloat16 [{N}], got {weight.dtype} {tuple(weight.shape)}")
+        rp, rl = residual.data_ptr(), _rows(residual, "residual", shape, bf16, device)
+        hp, hl = residual_out.data_ptr(), _rows(residual_out, "residual_out", shape, bf16, device)
+    if weight is not None:
+        wp = weight.data_ptr()
+        if weight.dtype != bf16 or weight.shape != (N,) or not weight.is_contiguous() or weight.get_device() != device:
+            raise XfError(3, f"weight: expected contiguous bfloat16 [{N}] on cuda:{device}, got {weight.dtype} "
+                             f"{tuple(weight.shape)} on {weight.device}")
     status = lib().xf_rms_norm_quantize(
-        _QUANTIZE_DESC.pack(out.data_ptr(), scale.data_ptr(), inp.data_ptr(), rp, hp,
-                            weight.data_ptr() if weight is not None else 0, ol, sr, sb, il, rl, hl, code, M, N, eps, 0, 0),
-        _stream())
+        _QUANTIZE_DESC.pack(out.data_ptr(), scale.data_ptr(), inp.data_ptr(), rp, hp, wp, ol, sr, sb, il, rl, hl, code,
+                            M, N, eps, 0, 0), torch._C._cuda_getCurrentRawStream(device))
     if status:
         check(status)
 
@@ -569,14 +567,13 @@ def rms_norm_quantize(out, scale, inp, weight=None, residual=None, residual_out=
 def act_mul_quantize(out, scale, inp, gelu=False):
     """out, scale = 8-bit act(inp[:, :d]) * inp[:, d:]; inp [M, 2d]; out and scale as in rms_norm_quantize."""
     import torch
-    shape = out.shape
+    shape, device = out.shape, torch.cuda.current_device()
     M, d = shape
-    _on_current_device(out, scale, inp)
-    code, sr, sb = _codes(out, scale)
-    il, ol = _rows(inp, "inp", (M, 2 * d), torch.bfloat16), _rows(out, "out", shape, out.dtype)
+    code, ol, sr, sb = _codes(out, scale, shape, device)
+    il = _rows(inp, "inp", (M, 2 * d), torch.bfloat16, device)
     status = lib().xf_act_mul_quantize(
         _QUANTIZE_DESC.pack(out.data_ptr(), scale.data_ptr(), inp.data_ptr(), 0, 0, 0, ol, sr, sb, il, 0, 0, code, M, d,
-                            0.0, 1 if gelu else 0, 0), _stream())
+                            0.0, 1 if gelu else 0, 0), torch._C._cuda_getCurrentRawStream(device))
     if status:
         check(status)
 

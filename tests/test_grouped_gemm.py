@@ -245,6 +245,21 @@ def test_no_rows(capi, cuda):
 
 
 @pytest.mark.gpu
+def test_status_is_reported_once(capi, cuda):
+    """A code in the status word, as a wait that gave up leaves one, is an error at the next query and then gone."""
+    op = make(20, 300, 9000)
+    plan, D = run(capi, op)
+    plan.workspace[:4].view(torch.int32).fill_(3)
+    torch.cuda.synchronize()
+    with pytest.raises(capi.XfError, match="device code 3"):
+        plan.device_status()
+    assert plan.device_status() == 0
+    plan.run()
+    torch.cuda.synchronize()
+    check(op, D, "none", D)
+
+
+@pytest.mark.gpu
 def test_plans_on_two_streams(capi, cuda):
     """Two plans with workspaces of their own, whose tiles are shared between CTAs, run at once."""
     ops = [make(40, 700, 8000, seed=s) for s in (1, 2)]

@@ -553,10 +553,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
             slot[i * 32] = make_float4(lo_of(sum[2 * i]), hi_of(sum[2 * i]), lo_of(sum[2 * i + 1]), hi_of(sum[2 * i + 1]));
         }
         __syncwarp();
-        if (live && lane == 0) {
-          __threadfence();
-          *reinterpret_cast<volatile int*>(p.flags + blockIdx.x * 8 + (warp - 4)) = 1;
-        }
+        if (live && lane == 0) ptx::st_release_gpu(p.flags + blockIdx.x * 8 + (warp - 4), 1);
         live = false;
       } else if (it.kb0 > 0 && live) {
         // The tile's last blocks: the units below hold the rest, nearest first, down to the one with block 0.
@@ -566,6 +563,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         // one lane for each of them, all flags at once; then their sums, nearest unit first
         int* flag = p.flags + ((unit - 1 - min(lane, count - 1)) * CTAS + static_cast<int>(rank)) * 8 + (warp - 4);
         w.wait_flags(flag, DEV_TIMEOUT_SPLIT_PARTIALS);
+        __syncwarp();                            // what one lane's flag announces is read by all
 #pragma unroll 1
         for (int u = 1; u <= count; ++u) {
           const int cta = (unit - u) * CTAS + static_cast<int>(rank);

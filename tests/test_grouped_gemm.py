@@ -286,6 +286,7 @@ def test_feed_forward_in_8_bits(capi, cuda, experts):
     gate_up, down = make(M, 2 * F, H, sizes, seed=1), make(M, H, F, sizes, nk=True, seed=2)
     off = gate_up.get("offsets")
     x = torch.randn(M, H, device=cuda).to(torch.bfloat16)
+    first_x = x.clone()
     res = torch.randn(M, H, device=cuda).to(torch.bfloat16)
     w = torch.rand(H, device=cuda).to(torch.bfloat16)
     h = torch.empty_like(x)
@@ -313,6 +314,21 @@ def test_feed_forward_in_8_bits(capi, cuda, experts):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(first, y)
+    # new inputs without a pause between the calls: no kernel reads what an earlier one left in a cache
+    xs = [torch.randn(M, H, device=cuda).to(torch.bfloat16) for _ in range(12)]
+    def all_of(wait):
+        got = []
+        for v in xs:
+            x.copy_(v)
+            layer()
+            got.append(y.clone())
+            if wait:
+                torch.cuda.synchronize()
+        return got
+    for one, other in zip(all_of(True), all_of(False)):
+        assert torch.equal(one, other)
+    x.copy_(first_x)
+    layer()
     # against the same layer in 64 bits without any quantisation: 8-bit steps of 2^-4 at three places
     ends = off.tolist() if experts else [0, M]
     n = h.double() / torch.sqrt(h.double().square().mean(1, keepdim=True) + 1e-6) * w.double()

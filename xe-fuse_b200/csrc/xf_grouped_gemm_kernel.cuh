@@ -51,7 +51,8 @@ struct alignas(64) Params {
   long long sa_row, sa_blk, sb_k, sb_n, sb_group;
   void* D;
   long long ldd;
-  int d_f32, pair, vec_d;
+  int d_f32, pair;
+  int vec_d;             // rows of D start on 16-byte boundaries: TMA may write them
   int* status;
   long long wait_budget;
   // Tiles whose K range several units share (split_kb > 0: see Split): one flag per epilogue warp and one
@@ -86,7 +87,7 @@ struct Cfg {
   static constexpr int LIST_BYTES = kTileList * 16;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 8 * STG_BYTES + BAR_BYTES + LIST_BYTES + TAB_BYTES;
   static_assert(BN_CTA % 128 == 0, "B is loaded in boxes of 128 columns");
-  static_assert(NC % 64 == 0 && NC <= 128, "an epilogue warp's columns share one scale of B");
+  static_assert(NC == 64 || NC == 128, "an epilogue warp's columns share one scale of B");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 };
 

@@ -203,10 +203,11 @@ struct Waiter {
   }
 };
 
-// Read-only 4-byte load that the compiler may not move to where its value is used.
+// 4-byte load that the compiler may not move to where its value is used.  Not the non-coherent form: with
+// programmatic dependent launch this kernel may have started before the one that writes the value ended.
 __device__ __forceinline__ float ld_early(const float* p) {
   float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
   return v;
 }
 

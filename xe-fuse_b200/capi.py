@@ -508,13 +508,13 @@ _QUANTIZE_DESC = struct.Struct("=6Q6q3ifii")
 def _rows(t, what, shape, dtype, device):
     """Checks a matrix with contiguous columns on the current device and returns its row pitch."""
     st = t.stride()
-    if t.dtype != dtype:
-        raise XfError(2, f"{what}: expected {dtype}, got {t.dtype}")
-    if t.shape != shape or (st[1] != 1 and shape[1] > 1):
-        raise XfError(3, f"{what}: expected a {tuple(shape)} tensor with contiguous columns, got "
-                         f"{tuple(t.shape)} with strides {st}")
-    if t.get_device() != device:
-        raise XfError(4, f"{what}: on {t.device}, but the current device is {device}")
+    if (t.dtype, t.shape, t.get_device()) != (dtype, shape, device) or (st[1] != 1 and shape[1] > 1):
+        if t.dtype != dtype:
+            raise XfError(2, f"{what}: expected {dtype}, got {t.dtype}")
+        if t.get_device() != device:
+            raise XfError(4, f"{what}: on {t.device}, but the current device is {device}")
+        raise XfError(3, f"{what}: expected a {tuple(shape)} tensor with contiguous columns, got {tuple(t.shape)} with "
+                         f"strides {st}")
     return st[0] if shape[0] > 1 else -(-shape[1] // 16) * 16    # a single row's pitch is of no use
 
 
@@ -528,10 +528,9 @@ def _codes(out, scale, shape, device):
         code, want = DT_S8, (M,)
     else:
         raise XfError(2, f"out: int8 or float8_e4m3fn, got {dtype}")
-    if scale.dtype != torch.float32 or scale.shape != want:
-        raise XfError(3, f"scale: expected float32 {want}, got {scale.dtype} {tuple(scale.shape)}")
-    if scale.get_device() != device:
-        raise XfError(4, f"scale: on {scale.device}, but the current device is {device}")
+    if (scale.dtype, scale.shape, scale.get_device()) != (torch.float32, want, device):
+        raise XfError(3, f"scale: expected float32 {want} on device {device}, got {scale.dtype} {tuple(scale.shape)} on "
+                         f"{scale.device}")
     # a dimension of one has no meaningful stride
     return (code, _rows(out, "out", shape, dtype, device), st[0] if M > 1 else 1,
             st[1] if N > 128 and code == DT_E4M3 else 1)
@@ -554,7 +553,7 @@ def rms_norm_quantize(out, scale, inp, weight=None, residual=None, residual_out=
         hp, hl = residual_out.data_ptr(), _rows(residual_out, "residual_out", shape, bf16, device)
     if weight is not None:
         wp = weight.data_ptr()
-        if weight.dtype != bf16 or weight.shape != (N,) or not weight.is_contiguous() or weight.get_device() != device:
+        if (weight.dtype, weight.shape, weight.get_device()) != (bf16, (N,), device) or not weight.is_contiguous():
             raise XfError(3, f"weight: expected contiguous bfloat16 [{N}] on cuda:{device}, got {weight.dtype} "
                              f"{tuple(weight.shape)} on {weight.device}")
     status = lib().xf_rms_norm_quantize(

@@ -11,8 +11,9 @@
 // of zeros zero codes and keeps L / a finite.  Maxima are taken over the bit patterns without the
 // sign, so a NaN is the largest of all and reaches the scale of its block.
 //
-// Bound.  All kernels move each byte once and are bound by HBM: 7 bytes per element with a residual
-// (x, r in; h, code out), 5 per output element of the gated form.
+// Bound.  Each byte moves once: 7 bytes per element with a residual (x, r in; h, code out), 5 per output
+// element of the gated form.  Long inputs run at 5.5 TB/s (4096 x 8192 42.5 us, 4096 x 14336 54 us), between HBM's
+// 6.5 and the issue slots' limit (about 21 instructions per column).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -69,6 +69,10 @@ struct Cfg {
   static constexpr int TM = 128 * CTAS;                 // rows of a tile
   static constexpr int ES = KIND == KIND_BF16 ? 2 : 1;
   static constexpr int KBLK = 128 / ES;                 // K elements of a stage: one 128-byte slab
+  // K blocks summed in TMEM before the sum moves to registers: one where each has its scales; with bf16 four (256
+  // elements), because the tensor core truncates as it adds: in one piece, K = 4236 to 7572 is 8e-6 of the
+  // result off, in pieces 2e-7 to 5e-7, like a sum of rounded products.  4096 x 4096 x 4096 takes 1 % longer.
+  static constexpr int SEG = KIND == KIND_E4M3 ? 1 : 4;
   static constexpr int UK = 32 / ES;                    // K elements of one MMA
   static constexpr int BN_CTA = BN / CTAS;              // columns of B one CTA loads
   static constexpr int GRP_COLS = 128 / ES;             // columns of a 128-byte column group ([K][N] weights)
@@ -418,8 +422,8 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       uint32_t phase = 0, tphase = 0;
       while (sched.next(p, *split, units, it)) {
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
-          const bool fresh = KIND == KIND_E4M3 || kb == it.kb0;          // starts an accumulator
-          const bool done = KIND == KIND_E4M3 || kb + 1 == it.kb1;       // and completes it
+          const bool fresh = (kb - it.kb0) % C::SEG == 0;                            // starts an accumulator
+          const bool done = (kb - it.kb0) % C::SEG == C::SEG - 1 || kb + 1 == it.kb1;   // and completes it
           w.wait(full0 + stage * 8, phase, DEV_TIMEOUT_MMA_FULL);
           const uint32_t sa = smem0 + stage * C::STAGE_BYTES;
           const uint64_t adesc = ptx::make_smem_desc_sw128(sa, 16, 1024);
@@ -490,7 +494,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       uint64_t sum[NC / 2];                    // columns 2 i and 2 i + 1
 #pragma unroll
       for (int i = 0; i < NC / 2; ++i) sum[i] = 0;
-      const int last = KIND == KIND_E4M3 ? it.kb1 - 1 : it.kb0;
+      const int last = it.kb1 - 1, segs = (it.kb1 - it.kb0 + C::SEG - 1) / C::SEG;
       auto open = [&]() {
         w.wait(tfull0 + buf * 8, tphase, DEV_TIMEOUT_EPI_TMEM_FULL);
         __syncwarp();
@@ -518,12 +522,13 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         }
       };
       if (!live) {                                // nothing to add, but every accumulator is released by all
-        for (int kb = it.kb0; kb <= last; ++kb) {
+        for (int s = 0; s < segs; ++s) {
           open();
           release();
         }
       } else if constexpr (KIND == KIND_BF16) {
-        take(1.0f);
+#pragma unroll 1
+        for (int s = 0; s < segs; ++s) take(1.0f);
       } else {
         // Block scales are asked for two blocks ahead of their use.
 #pragma unroll 1

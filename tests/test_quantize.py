@@ -122,6 +122,57 @@ def test_norm_special_rows(capi, cuda, s8):
     assert bool((scale[5] == 0).all()) and bool(torch.isfinite(q[5].float()).all())
 
 
+def nearest_quotient_e4m3(t, wide):
+    """Codes of t * 448 / wide: with 16 significant bits in t and `wide` a tie is exact in 64 bits, and no other quotient
+    comes nearer to one than 2^-21 of it."""
+    return nearest_e4m3(t * 448.0 / wide)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale_by", [2.0 ** -80, 1.0, 2.0 ** 100])
+def test_norm_e4m3_ties_go_to_even(capi, cuda, scale_by):
+    """Rows whose every quotient lies exactly between two codes: t = b w, largest value 448 b, quotient w."""
+    b = torch.arange(1, 256, 2, device=cuda, dtype=torch.float64)
+    m = torch.arange(17, 32, 2, device=cuda, dtype=torch.float64)
+    w = (m[:, None] * 2.0 ** torch.arange(-10, 4, device=cuda)).flatten()          # normal codes
+    w = torch.cat([w, (2 * torch.arange(8, device=cuda) + 1) * 2.0 ** -10])        # between subnormal codes
+    w = torch.cat([w, -w, w])[:254].view(2, 127)
+    w = torch.cat([torch.full((2, 1), 448.0, device=cuda, dtype=torch.float64), w], 1).flatten()
+    h = (b[:, None] * scale_by).expand(-1, w.numel()).to(torch.bfloat16).contiguous()
+    h[1::2] *= -1
+    assert torch.equal(h.double().abs(), (b[:, None] * scale_by).expand_as(h)) and torch.equal(w.to(torch.bfloat16).double(), w)
+    _, q, scale = out_tensors(len(b), w.numel(), False, 0)
+    capi.rms_norm_quantize(q, scale, h, w.to(torch.bfloat16), eps=0.0)
+    torch.cuda.synchronize()
+    want = nearest_e4m3(w) * torch.sign(h[:, :1].double())
+    assert torch.equal(q.double(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_e4m3_codes_are_the_exact_quotients(capi, cuda, residual):
+    """About 4 codes in 10000 of normal data are ties; N = 1000 ends in a short block."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.randn(512, 1000, device=cuda, generator=gen).to(torch.bfloat16)
+    x[0, 128:256] = float("inf")
+    x[0, 130] = -0.0
+    x[1, 5] = -0.0
+    w = torch.randn(1000, device=cuda, generator=gen).mul_(0.1).add_(1.0).to(torch.bfloat16)
+    res = torch.randn(512, 1000, device=cuda, generator=gen).to(torch.bfloat16) if residual else None
+    h = (x.float() + res.float()).to(torch.bfloat16) if residual else x
+    _, q, scale = out_tensors(512, 1000, False, 0)
+    capi.rms_norm_quantize(q, scale, x, w, res)
+    torch.cuda.synchronize()
+    t = h.double() * w.double()
+    _, wide = block_max(t, False)
+    fine = torch.isfinite(t) & torch.isfinite(wide)
+    assert torch.equal(q.double()[fine], nearest_quotient_e4m3(t, wide)[fine])
+    # the only finite value of a block of infinities has the code of zero, and zeros keep their sign
+    assert float(q[0, 130].float()) == 0.0
+    if not residual:
+        assert q.view(torch.int8)[0, 130] == -128 and q.view(torch.int8)[1, 5] == -128
+
+
 def gate_tolerance(g, gelu):
     if gelu:      # 1.5e-7 of a factor 1 + erf(z) that is at least 1 on the positive side; on the other
         #           side P(t) exp(-z^2) with |error of P| <= 1.5e-7 / exp(-z^2) of P(0) = 1

@@ -145,6 +145,27 @@ def test_outputs(capi, cuda, dtype_d, pair, extra, dtype):
         run(capi, op, dtype_d, pair, extra=extra, flags=flags)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [E4M3, torch.bfloat16])
+def test_geglu_of_negative_gates_keeps_its_relative_precision(capi, cuda, dtype):
+    """Gates and factors that the product gives exactly (one-hot rows); errors as for the row pass, in units of U:
+    __expf(g^2 / 2) 2 (2 + 1.173 g^2 / 2), the square and its exponent one rounding each, seen g^2 / 2 times larger, the
+    rest of the activation 8, the reciprocal 8, the product with the factor 1."""
+    K, pairs = 128, 72
+    gate = -(1.25 + torch.arange(pairs, device=cuda).double() / 8).view(1, -1).expand(K, -1)
+    gate = gate.to(dtype if dtype == E4M3 else torch.bfloat16).float()
+    factor = torch.tensor([0.5, -1.0, 1.75], device=cuda)[torch.arange(pairs, device=cuda) % 3].expand(K, -1)
+    B = torch.stack([gate, factor], 2).view(K, 2 * pairs).to(dtype)
+    A = torch.eye(K, device=cuda)[:40].to(dtype)
+    D = torch.empty(40, pairs, device=cuda)
+    one = dict(scale_a=torch.ones(40, 1, device=cuda), scale_b=torch.ones(1, 2, device=cuda)) if dtype == E4M3 else {}
+    capi.GroupedGemmPlan(A, B, D, pair="geglu", **one).run()
+    torch.cuda.synchronize()
+    g = gate[:40].double()
+    want = g * torch.exp(torch.special.log_ndtr(g)) * factor[:40].double()
+    assert bool(((D.double() - want).abs() <= (2 * (2 + 1.173 * g.square() / 2) + g.square() + 17) * U * want.abs()).all())
+
+
 GROUPS = [([5], 5, 0), ([0, 3, 0, 0, 9, 1, 0], 13, 0), ([130, 1, 127, 128, 129], 515, 0), ([0, 0, 0], 4, 0), ([2, 3], 20, 7),
           ([300, 0, 2, 700], 1100, 40), ([1] * 70, 70, 0), ([0] * 1023 + [33], 33, 0), ([1, 0] * 512, 512, 0)]
 

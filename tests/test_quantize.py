@@ -215,6 +215,33 @@ def test_act(capi, cuda, M, d, gelu, s8, extra):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("s8", [False, True])
+@pytest.mark.parametrize("d", [1, 3, 130, 257])
+def test_gelu_of_negative_gates_keeps_its_relative_precision(capi, cuda, d, s8):
+    """A block of nothing but strongly negative gates has a scale of its own.  Errors in units of u: __expf(g^2 / 2)
+    2 (2 + 1.173 g^2 / 2), the rest of the activation 8, the reciprocal 2 ulp, passed on 2.7 times at most: 8 more
+    than the exact one counted before, products with `up` and 1 / L 2."""
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    g = (torch.rand(64, d, device=cuda, generator=gen) * 8.5 + 2.5).neg().to(torch.bfloat16)
+    g[:5, -1] = torch.tensor([-4.0, -5.0, -8.0, -10.0, -11.0], device=cuda).to(torch.bfloat16)
+    u = (torch.rand(64, d, device=cuda, generator=gen) + 0.5).to(torch.bfloat16)
+    _, q, scale = out_tensors(64, d, s8, 0)
+    capi.act_mul_quantize(q, scale, torch.cat([g, u], 1), True)
+    torch.cuda.synchronize()
+    gd = g.double()
+    y = gd * torch.exp(torch.special.log_ndtr(gd)) * u.double()
+    slack = (2 * (2 + 1.173 * gd.square() / 2) + 18) * U * y.abs()
+    L = 127.0 if s8 else 448.0
+    a, _ = block_max(y, s8)
+    most, _ = block_max(slack, s8)
+    assert bool(((scale.double() * L - a).abs() <= most + 2 * U * a).all())
+    wide = scale.double()[:, None].expand_as(y) if s8 else scale.double().repeat_interleave(128, 1)[:, :d]
+    v = (y / wide).abs()
+    half = 0.5 if s8 else torch.exp2(torch.floor(torch.log2(v.clamp_min(2.0 ** -6))) - 4)
+    assert bool(((q.double() * wide - y).abs() <= half * wide * (1 + 2.0 ** -20) + 2 * slack + 4 * U * y.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("s8", [False, True])
 def test_act_special_values(capi, cuda, s8):
     d = 256
     x = torch.randn(4, 2 * d, device=cuda).to(torch.bfloat16)

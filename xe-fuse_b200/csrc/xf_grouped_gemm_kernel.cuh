@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
             for (int i = 0; i < UNIT / 2; ++i) v[i] = silu_fast(lo_of(s[i])) * hi_of(s[i]);
           } else {
 #pragma unroll
-            for (int i = 0; i < UNIT / 2; ++i) v[i] = gelu_f(lo_of(s[i])) * hi_of(s[i]);
+            for (int i = 0; i < UNIT / 2; ++i) v[i] = gelu_rel(lo_of(s[i])) * hi_of(s[i]);
           }
           uint32_t words[16];
 #pragma unroll

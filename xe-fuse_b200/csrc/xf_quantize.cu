@@ -329,7 +329,7 @@ __device__ __forceinline__ void gated(const Chunk& g, const Chunk& u, float (&y)
   unpack(g, a);
   unpack(u, b);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) y[i] = (GELU ? gelu_f(a[i]) : silu_fast(a[i])) * b[i];
+  for (int i = 0; i < 16; ++i) y[i] = (GELU ? gelu_rel(a[i]) : silu_fast(a[i])) * b[i];
 }
 
 // e4m3: kLanes lanes per block of 128 columns; nothing is shared beyond them.  A thread block works in one

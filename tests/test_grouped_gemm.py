@@ -296,6 +296,41 @@ def test_status_is_reported_once(capi, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("which", ["all", "one CTA", "one warp"])
+@pytest.mark.parametrize("shape", [(20, 300, 9000), (2100, 5200, 4096)])
+@pytest.mark.parametrize("dtype", [E4M3, torch.bfloat16])
+def test_a_wait_that_gives_up(capi, cuda, dtype, shape, which):
+    """The flags that say "partial sums are there" start so far below zero that they never rise above it: with short waits
+    the collecting warps give up after about a millisecond.  The launch ends (2100 x 5200: every unit has whole tiles
+    behind the shared one, so the other roles' waits run out as well, at different blocks), the status is reported
+    once, and the plan then runs as before."""
+    op = make(*shape, dtype=dtype)
+    D = torch.empty(shape[0], shape[1], device=cuda)
+    for flags in [0] + [f for f in tiles(capi, dtype)[1:] if not f & capi.FLAG_NO_SPLIT]:
+        plan = capi.GroupedGemmPlan(op["A"], op["B"], D, scale_a=op.get("scale_a"), scale_b=op.get("scale_b"),
+                                    flags=flags | capi.FLAG_SHORT_WAITS)
+        plan.run()
+        torch.cuda.synchronize()
+        assert plan.device_status() == 0
+        good = D.clone()
+        words = plan.workspace[256:].view(torch.int32)
+        words[:{"all": 148 * 8, "one CTA": 8, "one warp": 1}[which]] = -1000000
+        torch.cuda.synchronize()
+        plan.run()
+        torch.cuda.synchronize()                                 # returns: every wait is bounded
+        with pytest.raises(capi.XfError, match="device code [1-5]"):
+            plan.device_status()
+        assert plan.device_status() == 0
+        for _ in range(2):
+            D.fill_(-7.0)
+            plan.run()
+            torch.cuda.synchronize()
+            assert plan.device_status() == 0
+            assert torch.equal(D, good)
+    check(op, good, "none", good)
+
+
+@pytest.mark.gpu
 def test_plans_on_two_streams(capi, cuda):
     """Two plans with workspaces of their own, whose tiles are shared between CTAs, run at once."""
     ops = [make(40, 700, 8000, seed=s) for s in (1, 2)]

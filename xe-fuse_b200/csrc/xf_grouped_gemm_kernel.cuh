@@ -59,7 +59,7 @@ struct alignas(64) Params {
   // slot of partial sums per CTA.
   int split_kb;          // what sharing a tile between two units costs, in K blocks of one unit
   int split_max;         // most units that share a tile: they are summed one by one
-  int* flags;            // [grid][8], zero between launches
+  int* flags;            // [grid][8], zero between launches, raised by one
   float4* partials;      // [grid][8 warps][columns of a warp / 4][32 lanes]
 };
 
@@ -160,6 +160,19 @@ struct Split {
     hi = bound(rest * p.num_kb, n, unit + 1);
   }
 };
+// What the roles of a CTA have begun, for its end where a wait has run out.
+struct Begun {
+  int gave_up;          // a role of this CTA, or of the other one of a pair, did
+  int sent, sent_other; // K blocks copied here, and by the other CTA (known to the leader)
+  int issued, filled;   // K blocks multiplied, accumulators handed over (known to both)
+};
+// Waits until the last of `uses` completions of a ring of N barriers, one after another, has arrived at each of them.
+template <int N>
+__device__ __forceinline__ void wait_ring(uint64_t* ring, int uses, long long budget) {
+#pragma unroll 1
+  for (int s = 0; s < N && s < uses; ++s)
+    ptx::mbar_wait(ptx::smem_u32(&ring[s]), static_cast<uint32_t>((uses - 1 - s) / N) & 1u, budget);
+}
 // A role's walk over them; the split stays in shared memory, out of the role's registers.
 struct Walk {
   int next_tile, pos, count;   // count: items taken, the place of the next one's tile in the list
@@ -252,11 +265,13 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   using C = Cfg<KIND, BN, CTAS>;
   constexpr int STAGES = C::STAGES, NBUF = C::NBUF, NC = C::NC;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ Begun begun;
   const uint32_t raw = ptx::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   uint8_t* staging = smem + STAGES * C::STAGE_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 8 * C::STG_BYTES);
-  uint64_t* full_bar = bars;                     // [STAGES] operands landed (the leader CTA's is used)
+  uint64_t* full_bar = bars;                     // [STAGES] operands landed (the leader CTA's is used; each CTA of a pair
+                                                 //          announces and counts its own copies there)
   uint64_t* empty_bar = bars + STAGES;           // [STAGES] MMAs have read the stage
   uint64_t* tfull_bar = bars + 2 * STAGES;       // [NBUF]   accumulator complete
   uint64_t* tempty_bar = tfull_bar + NBUF;       // [NBUF]   accumulator read out (the leader CTA's is used)
@@ -278,7 +293,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   }
   if (warp == 1 && lane == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), CTAS);
       ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
     }
     for (int b = 0; b < NBUF; ++b) {
@@ -286,6 +301,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       ptx::mbar_init(ptx::smem_u32(&tempty_bar[b]), 8 * CTAS);
     }
     ptx::fence_mbar_init();
+    begun.gave_up = 0;
   }
   if (warp == 2) {
     ptx::tmem_alloc<CTAS>(ptx::smem_u32(tmem_slot), 512);
@@ -346,7 +362,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   const uint32_t tmem = ptx::uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
   Walk sched = {unit, ptx::uniform(split->hi), 0};
   Item it;
-  ptx::Waiter<Params> w = {p, false};
+  ptx::Waiter<Params> w = {p, &begun.gave_up, false};
 
   // 128 sums and two slices of 16 columns per thread do not fit the 168 registers that 384 threads can have
   // each: the first four warps hand theirs over (72 + 2 x 216 = 3 x 168).
@@ -355,29 +371,25 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   }
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    int stage = 0;
+    int stage = 0, sent = 0;
     uint32_t phase = 0;
     while (sched.next(p, *split, units, it)) {
       const Tile x = sched.count <= listed ? list[sched.count - 1] : decode<C>(p, first, grow, it.tile);
-      // rows of A that this CTA needs, and the bytes that both CTAs of a pair load
-      uint32_t bytes = 0;
-      int boxes = 0;                             // of 32 rows; 4: one box of 128
-#pragma unroll
-      for (int c = 0; c < CTAS; ++c) {
-        const int need = min(max((x.rows - c * 128 + 31) / 32, 0), 4);
-        bytes += need * 4096 + C::B_BYTES;
-        if (c == static_cast<int>(rank)) boxes = need;
-      }
+      // rows of A that this CTA needs, in boxes of 32 (4: one box of 128), and the bytes that it loads
+      const int boxes = min(max((x.rows - static_cast<int>(rank) * 128 + 31) / 32, 0), 4);
+      const uint32_t bytes = boxes * 4096 + C::B_BYTES;
       const int row = x.row0 + static_cast<int>(rank) * 128;
       const int col = x.n0 + static_cast<int>(rank) * C::BN_CTA;
       const int bg = p.b_grouped ? x.g : 0;
       for (int kb = it.kb0; kb < it.kb1; ++kb) {
         w.wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, DEV_TIMEOUT_PRODUCER_EMPTY);
         // once a wait has run out nothing more is loaded: a stage's barrier may still be in its last phase
-        if (!w.any_lost() && ptx::elect_one()) {
+        const bool go = !w.any_lost();
+        if (go && ptx::elect_one()) {
           const uint32_t own = ptx::smem_u32(&full_bar[stage]);
           const uint32_t bar = CTAS == 2 ? ptx::mapa(own, 0) : own;
-          if (rank == 0) ptx::mbar_arrive_expect_tx(own, bytes);
+          if constexpr (CTAS == 2) ptx::mbar_arrive_expect_tx_cluster(bar, bytes);
+          else ptx::mbar_arrive_expect_tx(own, bytes);
           const uint32_t sa = ptx::smem_u32(smem + stage * C::STAGE_BYTES), sb = sa + C::A_BYTES;
           const int k = kb * C::KBLK;
           if (boxes == 4) {
@@ -396,15 +408,16 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
           }
         }
         __syncwarp();
+        sent += go;
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
     }
-    // The CTA may not go before its last copies have landed, also where another role gave up and nobody
-    // waited for them (the leader's barriers count both CTAs' bytes; the pair leaves together).
-    if (rank == 0) {
-      for (int s = 0; s < STAGES; ++s)
-        w.wait(ptx::smem_u32(&full_bar[s]), s < stage ? phase : phase ^ 1u, DEV_TIMEOUT_MMA_FULL);
-    }
+    // The last stages have been read, so their copies have landed, and the commits that say so have arrived here.
+    // (Rolled up: code that runs once comes cold from memory; unrolled, the loops here took 0.5 us.)
+#pragma unroll 1
+    for (int s = 0; s < STAGES; ++s)
+      w.wait(ptx::smem_u32(&empty_bar[s]), s < stage ? phase : phase ^ 1u, DEV_TIMEOUT_PRODUCER_EMPTY);
+    if (lane == 0) begun.sent = sent;
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     // The whole warp walks the loop and one elected lane issues: addresses and descriptors then stay in
@@ -418,7 +431,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
       const uint64_t b_step = p.b_nk ? 2u : static_cast<uint64_t>(C::UK * 128) >> 4;   // per MMA, in 16 bytes
       const uint32_t smem0 = ptx::smem_u32(smem), full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
       const uint32_t tfull0 = ptx::smem_u32(tfull_bar), tempty0 = ptx::smem_u32(tempty_bar);
-      int stage = 0, buf = 0;
+      int stage = 0, buf = 0, issued = 0, filled = 0;
       uint32_t phase = 0, tphase = 0;
       while (sched.next(p, *split, units, it)) {
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
@@ -447,11 +460,21 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
             }
           }
           __syncwarp();
+          issued += !lost;
+          filled += done && !lost;
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
           if (done && ++buf == NBUF) { buf = 0; tphase ^= 1u; }
         }
       }
-    }
+      // The last accumulators have been read, and the other CTA's arrivals that say so have come in.
+#pragma unroll 1
+      for (int b = 0; b < NBUF; ++b)
+        w.wait(tempty0 + b * 8, b < buf ? tphase : tphase ^ 1u, DEV_TIMEOUT_MMA_TMEM_EMPTY);
+      if (lane == 0) {
+        begun.issued = issued;
+        begun.filled = filled;
+      }
+      }
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ promotion and epilogue
     if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -559,7 +582,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
             slot[i * 32] = make_float4(lo_of(sum[2 * i]), hi_of(sum[2 * i]), lo_of(sum[2 * i + 1]), hi_of(sum[2 * i + 1]));
         }
         __syncwarp();
-        if (live && lane == 0) ptx::st_release_gpu(p.flags + blockIdx.x * 8 + (warp - 4), 1);
+        if (live && lane == 0) ptx::add_release_gpu(p.flags + blockIdx.x * 8 + (warp - 4), 1);
         live = false;
       } else if (it.kb0 > 0 && live) {
         // The tile's last blocks: the units below hold the rest, nearest first, down to the one with block 0.
@@ -647,8 +670,52 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
   __syncthreads();
   // No CTA leaves while its peer may still write its barriers or read the pair's TMEM.
   if constexpr (CTAS > 1) {
+    if (threadIdx.x == 0 && begun.gave_up) {       // both learn of it
+      ptx::st_shared_cluster(ptx::mapa(ptx::smem_u32(&begun.gave_up), rank ^ 1u), 1);
+      ptx::fence_cluster();
+    }
+    __syncwarp();
     ptx::cluster_arrive_relaxed();
     ptx::cluster_wait();
+  }
+  if (begun.gave_up) {
+    // Roles that gave up stopped at different blocks, so copies, MMAs and commits may be on their way that nobody
+    // waited for.  What was begun says which of them have to arrive before the shared memory and TMEM may go.
+    if constexpr (CTAS > 1) {
+      if (warp == 0 && lane == 0) {
+        if (rank != 0) {
+          ptx::st_shared_cluster(ptx::mapa(ptx::smem_u32(&begun.sent_other), 0), begun.sent);
+        } else {
+          ptx::st_shared_cluster(ptx::mapa(ptx::smem_u32(&begun.issued), 1), begun.issued);
+          ptx::st_shared_cluster(ptx::mapa(ptx::smem_u32(&begun.filled), 1), begun.filled);
+        }
+      }
+      __syncwarp();
+      ptx::cluster_arrive();
+      ptx::cluster_wait();
+    }
+    if (warp == 0 && rank == 0) {
+      int sent = begun.sent;
+      if constexpr (CTAS > 1) {
+        // A block that only one CTA copied lacks the other one's announcement.  (One CTA is at most STAGES blocks ahead:
+        // a stage is filled again only after MMAs have read what both had put there.)
+        const int from = min(sent, begun.sent_other);
+        sent = max(sent, begun.sent_other);
+        for (int b = from + lane; b < sent; b += 32) ptx::mbar_arrive(ptx::smem_u32(&full_bar[b % STAGES]));
+        __syncwarp();
+      }
+      wait_ring<STAGES>(full_bar, sent, p.wait_budget);
+    } else if (warp == 1) {
+      wait_ring<STAGES>(empty_bar, begun.issued, p.wait_budget);
+      wait_ring<NBUF>(tfull_bar, begun.filled, p.wait_budget);
+    }
+    __syncwarp();
+    if constexpr (CTAS > 1) {
+      ptx::cluster_arrive();
+      ptx::cluster_wait();
+    } else {
+      __syncthreads();
+    }
   }
   if (warp == 2) {
     ptx::tc_fence_after();

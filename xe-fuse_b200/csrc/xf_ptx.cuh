@@ -51,8 +51,8 @@ __device__ __forceinline__ int ld_acquire_gpu(const int* p) {
   return v;
 }
 
-__device__ __forceinline__ void st_release_gpu(int* p, int v) {
-  asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+__device__ __forceinline__ void add_release_gpu(int* p, int v) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
 
 __device__ __forceinline__ uint32_t mapa(uint32_t smem_addr, uint32_t rank) {
@@ -97,6 +97,11 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_bar
 }
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+// The same for a barrier of the cluster, without memory ordering: it counts bytes, the copies themselves order the data.
+__device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes)
                : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
@@ -172,31 +177,34 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
 // A value that is the same in all lanes, known as such to the compiler.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
-// A role's bounded waits.  One that runs out writes its code to the status word and lets the role go on
-// without waiting again for long: the launch is lost, but every role still walks its whole list and control
-// flow does not depend on a wait's outcome (a loop that a wait may leave keeps its counters, and with them
-// the operands of tensor-core instructions, out of uniform registers).  P: kernel parameters with `status`
-// and `wait_budget`, which are read where they are needed and take no registers meanwhile.
+// A role's bounded waits.  One that runs out writes its code to the status word and raises the CTA's `gave_up`
+// (static shared memory: its address takes no register); from then on no role of the CTA waits for anything that is
+// not there.  The launch is lost, but every role still walks its whole list and control flow does not depend on a
+// wait's outcome (a loop that a wait may leave keeps its counters, and with them the operands of tensor-core
+// instructions, out of uniform registers).  P: kernel parameters with `status` and `wait_budget`, which are read
+// where they are needed and take no registers meanwhile.
 template <class P>
 struct Waiter {
   const P& p;
-  bool lost;
+  int* gave_up;
+  bool lost;             // for roles that begin nothing any more
+  __device__ __forceinline__ bool give_up(int code) {
+    if (p.status) atomicCAS(p.status, 0, code);
+    *reinterpret_cast<volatile int*>(gave_up) = 1;
+    return true;
+  }
   __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, int code) {
     if (mbar_try_wait(bar, parity)) return;
-    if (!mbar_wait(bar, parity, lost ? 0 : p.wait_budget)) {
-      if (p.status) atomicCAS(p.status, 0, code);
-      lost = true;
-    }
+    if (*reinterpret_cast<volatile int*>(gave_up) || (!mbar_wait(bar, parity, p.wait_budget) && give_up(code))) lost = true;
   }
   __device__ __forceinline__ bool any_lost() const { return __any_sync(0xffffffffu, lost); }
-  // Until other CTAs have set the flags that the lanes name; by a converged warp (a loop in one lane only
+  // Until other CTAs have raised the flags that the lanes name above zero; by a converged warp (a loop in one lane only
   // made the compiler spill what lives in registers around it).
   __device__ __forceinline__ void wait_flags(const int* flag, int code) {
     const long long t0 = clock64();
-    while (!__all_sync(0xffffffffu, ld_acquire_gpu(flag) != 0)) {
-      if (uniform(clock64() - t0 > (lost ? 0 : p.wait_budget))) {
-        if (p.status) atomicCAS(p.status, 0, code);
-        lost = true;
+    while (!__all_sync(0xffffffffu, ld_acquire_gpu(flag) > 0)) {
+      if (uniform(*reinterpret_cast<volatile int*>(gave_up) || clock64() - t0 > p.wait_budget)) {
+        give_up(code);
         break;
       }
     }
@@ -211,7 +219,11 @@ __device__ __forceinline__ float ld_early(const float* p) {
   return v;
 }
 
-// 16-byte store into the shared memory of another CTA of the cluster (address from mapa).
+// Stores into the shared memory of another CTA of the cluster (address from mapa).
+__device__ __forceinline__ void st_shared_cluster(uint32_t cluster_addr, int v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ void st_shared_cluster_v4(uint32_t cluster_addr, const uint4& v) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(v.x),
                "r"(v.y), "r"(v.z), "r"(v.w)

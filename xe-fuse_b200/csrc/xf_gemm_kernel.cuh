@@ -145,6 +145,8 @@ __device__ __forceinline__ WorkItem decode_item(const GemmParams& p, int w) {
   return it;
 }
 
+// Operands of the epilogue are read by plain loads, not through the non-coherent path (__ldg): with programmatic dependent
+// launch this kernel may have started before the one that writes them (a norm's residual stream, say) ended.
 __device__ __forceinline__ float load_vec_elem(const VecArg& v, long long idx) {
   if (v.ptr == nullptr) return v.null_default;
   if (v.dtype == DT_BF16)
@@ -167,7 +169,7 @@ __device__ __forceinline__ void load_vec32(const VecArg& a, int l, int col0, int
     if (col0 + 32 <= n_total && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(ptr) + j);
+        const uint4 u = reinterpret_cast<const uint4*>(ptr)[j];
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -184,7 +186,7 @@ __device__ __forceinline__ void load_vec32(const VecArg& a, int l, int col0, int
     if (col0 + 32 <= n_total && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(ptr) + j);
+        const float4 f = reinterpret_cast<const float4*>(ptr)[j];
         out[j * 4 + 0] = f.x; out[j * 4 + 1] = f.y; out[j * 4 + 2] = f.z; out[j * 4 + 3] = f.w;
       }
     } else {
@@ -212,7 +214,7 @@ __device__ __forceinline__ void apply_vec32(const VecArg& a, int l, int col0, in
     if (col0 + 32 <= n_total && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(ptr) + j);
+        const uint4 u = reinterpret_cast<const uint4*>(ptr)[j];
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -229,7 +231,7 @@ __device__ __forceinline__ void apply_vec32(const VecArg& a, int l, int col0, in
     if (col0 + 32 <= n_total && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(ptr) + j);
+        const float4 f = reinterpret_cast<const float4*>(ptr)[j];
         v[j * 4 + 0] = op(v[j * 4 + 0], f.x); v[j * 4 + 1] = op(v[j * 4 + 1], f.y);
         v[j * 4 + 2] = op(v[j * 4 + 2], f.z); v[j * 4 + 3] = op(v[j * 4 + 3], f.w);
       }
@@ -273,7 +275,7 @@ __device__ __forceinline__ int mat_row32_issue(const MatArg& m, int l, int row, 
     const __nv_bfloat16* ptr = reinterpret_cast<const __nv_bfloat16*>(m.ptr) + off;
     if (col0 + 32 <= ncols_total && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) raw[j] = __ldg(reinterpret_cast<const uint4*>(ptr) + j);
+      for (int j = 0; j < 4; ++j) raw[j] = reinterpret_cast<const uint4*>(ptr)[j];
       return 1;
     }
     return 2;
@@ -281,7 +283,7 @@ __device__ __forceinline__ int mat_row32_issue(const MatArg& m, int l, int row, 
   const float* ptr = reinterpret_cast<const float*>(m.ptr) + off;
   if (col0 + 32 <= ncols_total && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) raw[j] = __ldg(reinterpret_cast<const uint4*>(ptr) + j);
+    for (int j = 0; j < 8; ++j) raw[j] = reinterpret_cast<const uint4*>(ptr)[j];
     return 1;
   }
   return 2;

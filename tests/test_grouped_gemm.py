@@ -348,6 +348,94 @@ def test_plans_on_two_streams(capi, cuda):
         check(o, D, "none", D)
 
 
+def renew(op, other):
+    """Puts another operand set's values in place of this one's."""
+    for k in ("A", "B"):
+        if op[k].dtype == E4M3:
+            op[k].view(torch.int8).copy_(other[k].view(torch.int8))
+        else:
+            op[k].copy_(other[k])
+    for k in ("scale_a", "scale_b"):
+        if k in op:
+            op[k].copy_(other[k])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [E4M3, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K", [(20, 300, 9000), (400, 300, 9000), (2100, 1300, 4096)])
+def test_shared_tiles_meet_new_data(capi, cuda, dtype, M, N, K):
+    """Tiles whose K range several CTAs share, launch after launch with new operands and the old result overwritten: sums
+    that an earlier launch published, or a flag that it left raised, would show in the result."""
+    sets = [make(M, N, K, dtype=dtype, seed=s) for s in (1, 2, 3)]
+    op = make(M, N, K, dtype=dtype, seed=4)
+    D = torch.empty(M, N, device=cuda)
+    plans = [capi.GroupedGemmPlan(op["A"], op["B"], D, scale_a=op.get("scale_a"), scale_b=op.get("scale_b"), flags=f)
+             for f in tiles(capi, dtype) if not f & capi.FLAG_NO_SPLIT]
+    assert all(plan.workspace.numel() > 256 for plan in plans)       # they may share tiles
+    for plan in plans:
+        got = []
+        for i in (0, 1, 2, 1, 0):                                    # no pause: one launch's end meets the next one's start
+            renew(op, sets[i])
+            D.fill_(-7.0)
+            plan.run()
+            got.append((i, D.clone()))
+        assert plan.device_status() == 0
+        for i, D_i in got:
+            check(sets[i], D_i, "none", D_i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [E4M3, torch.bfloat16])
+def test_routing_of_shared_tiles_changes_under_a_graph(capi, cuda, dtype):
+    """K = 8000 and few row tiles: every launch shares its tiles, other ones each time, among other CTAs."""
+    M, N, K = 300, 264, 8000
+    sets = [make(M, N, K, [75] * 4, dtype, seed=s) for s in (1, 2)]
+    for flags in tiles(capi, dtype):
+        if flags & capi.FLAG_NO_SPLIT:
+            continue
+        op = make(M, N, K, [75] * 4, dtype, seed=3)
+        D = torch.zeros(M, N, device=cuda)
+        plan = capi.GroupedGemmPlan(op["A"], op["B"], D, offsets=op["offsets"], scale_a=op.get("scale_a"),
+                                    scale_b=op.get("scale_b"), flags=flags)
+        plan.run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.run()
+        for i, ends in enumerate(([0, 100, 100, 250, 300], [0, 0, 0, 0, 300], [0, 1, 2, 3, 4], [10, 10, 200, 201, 290],
+                                  [5, 5, 5, 5, 5], [0, 299, 299, 299, 300], [0, 100, 100, 250, 300])):
+            renew(op, sets[i % 2])
+            op["offsets"].copy_(torch.tensor(ends, dtype=torch.int32))
+            D.fill_(-7.0)
+            before = D.clone()
+            graph.replay()
+            check(op, D, "none", before)
+        assert plan.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_plans_on_two_streams_meet_new_data(capi, cuda):
+    """Two plans with workspaces of their own and shared tiles at once, each launch on other operands."""
+    sets = [[make(40, 700, 8000, seed=10 * p + s) for s in range(3)] for p in (1, 2)]
+    ops = [make(40, 700, 8000, seed=p) for p in (5, 6)]
+    outs = [torch.empty(40, 700, device=cuda) for _ in ops]
+    plans = [capi.GroupedGemmPlan(o["A"], o["B"], D, scale_a=o["scale_a"], scale_b=o["scale_b"]) for o, D in zip(ops, outs)]
+    streams = [torch.cuda.Stream() for _ in ops]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for step in range(9):
+        for p, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                renew(ops[p], sets[p][step % 3])
+                outs[p].fill_(-7.0)
+                plans[p].run()
+                got[p].append(outs[p].clone())
+    torch.cuda.synchronize()
+    for p in (0, 1):
+        assert plans[p].device_status() == 0
+        for step, D in enumerate(got[p]):
+            check(sets[p][step % 3], D, "none", D)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("experts", [False, True])
 def test_feed_forward_in_8_bits(capi, cuda, experts):

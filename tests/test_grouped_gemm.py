@@ -553,6 +553,16 @@ def test_refusals(capi, change, status):
     assert capi.lib().xf_grouped_gemm_can_implement(C.byref(desc(capi, **change))) == status
 
 
+@pytest.mark.parametrize("bf16,flags,status", [
+    (0, ("1CTA", "BN256"), 0), (0, ("2CTA", "BN256"), 0), (0, ("1CTA", "BN128"), 0), (0, ("BN128",), 0), (0, ("2CTA",), 0),
+    (0, ("2CTA", "BN128"), 5), (0, ("1CTA", "2CTA"), 5), (0, ("BN128", "BN256"), 5),
+    (1, ("2CTA", "BN256"), 0), (1, ("1CTA", "BN128"), 0), (1, ("1CTA", "BN256"), 5), (1, ("2CTA", "BN128"), 5)])
+def test_flags_that_leave_no_tile_are_refused_at_once(capi, bf16, flags, status):
+    word = sum(getattr(capi, "FLAG_FORCE_" + f) for f in flags)
+    more = dict(dtype_ab=0, scale_a=None, scale_b=None) if bf16 else {}
+    assert capi.lib().xf_grouped_gemm_can_implement(C.byref(desc(capi, flags=word, **more))) == status
+
+
 def test_null_arguments(capi):
     L = capi.lib()
     assert L.xf_grouped_gemm_can_implement(None) == 4

@@ -17,6 +17,15 @@ namespace grouped {
 
 static bool aligned(const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) % to) == 0; }
 
+static const Variant* tiles_of(int dtype_ab, int* count) {
+  *count = dtype_ab == XF_DT_BF16 ? kTilesBf16 : kTilesE4m3;
+  return dtype_ab == XF_DT_BF16 ? g_variants_bf16 : g_variants_e4m3;
+}
+static bool allowed(const Variant& v, int flags) {
+  return !((flags & XF_FLAG_FORCE_1CTA && v.ctas != 1) || (flags & XF_FLAG_FORCE_2CTA && v.ctas != 2) ||
+           (flags & XF_FLAG_FORCE_BN128 && v.bn != 128) || (flags & XF_FLAG_FORCE_BN256 && v.bn != 256));
+}
+
 static xf_status validate(const xf_grouped_gemm_desc* d) {
   if (!d) {
     set_error("null descriptor");
@@ -44,6 +53,13 @@ static xf_status validate(const xf_grouped_gemm_desc* d) {
   }
   if (d->flags & ~(XF_FLAG_FORCE_1CTA | XF_FLAG_FORCE_2CTA | XF_FLAG_FORCE_BN128 | XF_FLAG_FORCE_BN256 | XF_FLAG_NO_SPLIT | XF_FLAG_NO_PDL | XF_FLAG_SHORT_WAITS)) {
     set_error("unsupported flags 0x%x", d->flags);
+    return XF_ERR_NOT_SUPPORTED;
+  }
+  int count = 0, left = 0;
+  const Variant* all = tiles_of(d->dtype_ab, &count);
+  for (int i = 0; i < count; ++i) left += allowed(all[i], d->flags);
+  if (left == 0) {
+    set_error("no tile of this type matches the flags 0x%x", d->flags);
     return XF_ERR_NOT_SUPPORTED;
   }
   if (d->b_layout != XF_B_KN && d->b_layout != XF_B_NK) {
@@ -139,15 +155,14 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
   // 128 x 256 / 128 x 128: 4096 x 28672 x 4096 402 / 446 / 530 us, 777 x 5001 x 2000 34 / 20 / 24 us,
   // 64 experts 16384 x 4096 x 2048 262 / 215 / 236 us, 100 x 8192 x 8192 - / 23 / 16.5 us.
   const Variant* v = nullptr;
-  const Variant* all = kind == KIND_BF16 ? g_variants_bf16 : g_variants_e4m3;
-  const int count = kind == KIND_BF16 ? kTilesBf16 : kTilesE4m3, kblk = kind == KIND_BF16 ? 64 : 128;
+  int count = 0;
+  const Variant* all = tiles_of(d->dtype_ab, &count);
+  const int kblk = kind == KIND_BF16 ? 64 : 128;
   const double num_kb = (d->K + kblk - 1) / kblk;
   double best = 0.0;
   for (int i = 0; i < count; ++i) {
     const Variant& c = all[i];
-    if ((d->flags & XF_FLAG_FORCE_1CTA && c.ctas != 1) || (d->flags & XF_FLAG_FORCE_2CTA && c.ctas != 2) ||
-        (d->flags & XF_FLAG_FORCE_BN128 && c.bn != 128) || (d->flags & XF_FLAG_FORCE_BN256 && c.bn != 256))
-      continue;
+    if (!allowed(c, d->flags)) continue;
     const bool wide = c.bn == 256;
     const double per_kb = kind == KIND_BF16 ? (wide ? 680 : 490) : (c.ctas == 2 ? 720 : wide ? 870 : 600);
     const double tile = num_kb * per_kb + (wide ? 3700 : 2000), publish = wide ? 5000 : 3000, sum = wide ? 1800 : 900;
@@ -166,10 +181,6 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
       g->split_kb = static_cast<int>((publish + sum) / per_kb + 0.5);
       g->split_max = split_max;
     }
-  }
-  if (!v) {
-    set_error("no tile of this type matches the flags 0x%x", d->flags);
-    return XF_ERR_NOT_SUPPORTED;
   }
   const bool f32 = d->dtype_d == XF_DT_F32;
   g->fn = v->fn[d->pair == XF_PAIR_NONE ? (f32 ? OUT_F32 : OUT_BF16) : (f32 ? OUT_PAIR_F32 : OUT_PAIR_BF16)];

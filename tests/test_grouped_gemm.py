@@ -592,3 +592,23 @@ def test_wrapper_refusals(capi, monkeypatch):
     ):
         with pytest.raises(capi.XfError):
             capi.GroupedGemmPlan(*a, **k)
+
+
+def test_wrapper_refuses_types_and_shapes_in_its_own_manner(capi, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    A, B, D = torch.zeros(8, 256, dtype=E4M3), torch.zeros(256, 128, dtype=E4M3), torch.zeros(8, 128)
+    k = dict(scale_a=torch.ones(8, 2), scale_b=torch.ones(2, 1))
+    half = [t.to(torch.float16) for t in (A.float(), B.float())]
+    for a, more in (
+        ((A, B, D.half()), k),                                       # no such result
+        ((half[0], half[1], D), {}),                                 # nor such operands
+        ((A[0], B, D), k), ((A[None], B, D), k), ((A, B[0], D), k), ((A, B[None, None], D), k),
+        ((A, B, D[0]), k), ((A, B, D[None]), k),
+        ((A, B, D), dict(k, offsets=torch.zeros((), dtype=torch.int32))),
+        ((A, B, D), dict(k, offsets=torch.zeros(0, dtype=torch.int32))),
+        ((A, B, D), dict(k, offsets=torch.zeros(1, 2, dtype=torch.int32))),
+        ((A, B, D), dict(k, pair="relu")),
+        ((A, B, D), dict(k, scale_a=torch.ones(8))),
+    ):
+        with pytest.raises(capi.XfError):
+            capi.GroupedGemmPlan(*a, **more)

@@ -368,3 +368,19 @@ def test_wrapper_refusals(capi, monkeypatch):
     ):
         with pytest.raises(capi.XfError):
             bad()
+
+
+def test_wrapper_refuses_other_dimensions_in_its_own_manner(capi, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    x, s, q = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(4, 2), torch.zeros(4, 256, dtype=E4M3)
+    for bad in (
+        lambda: capi.rms_norm_quantize(q[0], s[0], x[0]),
+        lambda: capi.rms_norm_quantize(q[None], s[None], x[None]),
+        lambda: capi.rms_norm_quantize(q, s, x[0]),
+        lambda: capi.rms_norm_quantize(q, s, x, x[:1]),              # weight is a vector
+        lambda: capi.act_mul_quantize(q[0], s[0], x[0]),
+        lambda: capi.act_mul_quantize(q[:, :128], s[:, :1], x[None]),
+        lambda: capi.act_mul_quantize(q[:, :128], s[0, :1], x),
+    ):
+        with pytest.raises(capi.XfError):
+            bad()

@@ -180,8 +180,11 @@ def check(status):
 
 def _torch_dtype_code(t):
     import torch
-    return {torch.bfloat16: DT_BF16, torch.int8: DT_S8, torch.float32: DT_F32, torch.int32: DT_S32,
-            torch.float8_e4m3fn: DT_E4M3}[t.dtype]
+    code = {torch.bfloat16: DT_BF16, torch.int8: DT_S8, torch.float32: DT_F32, torch.int32: DT_S32,
+            torch.float8_e4m3fn: DT_E4M3}.get(t.dtype)
+    if code is None:
+        raise XfError(2, f"no operand type is {t.dtype}")
+    return code
 
 
 def vec(t, batch_stride=0, null_default=1.0):
@@ -305,6 +308,11 @@ class GroupedGemmPlan:
                 raise XfError(4, f"tensor on {t.device}, but the current device is cuda:{device}")
         if B.dtype != A.dtype:
             raise XfError(2, f"A and B must have one type, got {A.dtype} and {B.dtype}")
+        if A.dim() != 2 or B.dim() not in (2, 3) or (offsets is not None and offsets.dim() != 1):
+            raise XfError(3, "expected A [M, K], B of 2 or 3 dimensions and a vector of offsets, got " +
+                          ", ".join(str(tuple(t.shape)) for t in (A, B, offsets) if t is not None))
+        if pair not in PAIR:
+            raise XfError(4, f"no pair op {pair!r}")
         M, K = A.shape
         N = B.shape[-2] if b_nk else B.shape[-1]
         G = offsets.shape[0] - 1 if offsets is not None else 1
@@ -313,7 +321,7 @@ class GroupedGemmPlan:
         ldd = _rows(D, "D", (M, N if pair == "none" else N // 2), D.dtype, device)
         if tuple(B.shape) != lead + ((N, K) if b_nk else (K, N)) or (B.shape[-1] > 1 and B.stride(-1) != 1):
             raise XfError(3, f"B: {tuple(B.shape)} with strides {B.stride()} does not fit A {tuple(A.shape)} and {G} groups")
-        if offsets is not None and (offsets.dtype != torch.int32 or offsets.dim() != 1 or not offsets.is_contiguous()):
+        if offsets is not None and (offsets.dtype != torch.int32 or not offsets.is_contiguous()):
             raise XfError(2, "offsets: contiguous int32 vector expected")
         d = XfGroupedGemmDesc()
         d.dtype_ab, d.dtype_d = _torch_dtype_code(A), _torch_dtype_code(D)
@@ -521,6 +529,8 @@ def _rows(t, what, shape, dtype, device):
 def _codes(out, scale, shape, device):
     """(type, row pitch, row stride and block stride of the scales) of an 8-bit output."""
     import torch
+    if len(shape) != 2:
+        raise XfError(3, f"expected a matrix, got shape {tuple(shape)}")
     dtype, (M, N), st = out.dtype, shape, scale.stride()
     if dtype == torch.float8_e4m3fn:
         code, want = DT_E4M3, (M, -(-N // 128))
@@ -542,8 +552,8 @@ def rms_norm_quantize(out, scale, inp, weight=None, residual=None, residual_out=
     strides (the block-scaled products read fastest with the rows side by side: torch.empty(blocks, M).t())."""
     import torch
     shape, bf16, device = inp.shape, torch.bfloat16, torch.cuda.current_device()
-    M, N = shape
     code, ol, sr, sb = _codes(out, scale, shape, device)
+    M, N = shape
     il = _rows(inp, "inp", shape, bf16, device)
     rp = hp = rl = hl = wp = 0
     if residual is not None:
@@ -567,8 +577,8 @@ def act_mul_quantize(out, scale, inp, gelu=False):
     """out, scale = 8-bit act(inp[:, :d]) * inp[:, d:]; inp [M, 2d]; out and scale as in rms_norm_quantize."""
     import torch
     shape, device = out.shape, torch.cuda.current_device()
-    M, d = shape
     code, ol, sr, sb = _codes(out, scale, shape, device)
+    M, d = shape
     il = _rows(inp, "inp", (M, 2 * d), torch.bfloat16, device)
     status = lib().xf_act_mul_quantize(
         _QUANTIZE_DESC.pack(out.data_ptr(), scale.data_ptr(), inp.data_ptr(), 0, 0, 0, ol, sr, sb, il, 0, 0, code, M, d,

@@ -374,7 +374,7 @@ XF_API xf_status xf_ve_dequant_rotary(void* out, const int32_t* acc, const float
  * scale[m * scale_row_stride + b * scale_blk_stride].  Maxima are floored at 2^-100 times the row's
  * rstd, so zeros get zero codes and a finite scale; a NaN or an infinity makes the scale of its block
  * NaN or infinite.  Pitches in elements, any value from the row's width up and any alignment; 16-byte
- * aligned rows are faster.  N up to 2^20.  M == 0 is an empty call.  All asynchronous on
+ * aligned rows are faster (and the products need them: see below).  N up to 2^20.  M == 0 is an empty call.  All asynchronous on
  * `stream`, of the current device; no workspace.
  */
 typedef struct xf_quantize_desc {
@@ -410,6 +410,10 @@ XF_API xf_status xf_act_mul_quantize(const xf_quantize_desc* desc, void* stream)
  *                                          + (n / 128) * scale_b_n_stride]
  * scale_a is read fastest with a row stride of 1.
  *
+ * A and B are read in 16-byte units: their base addresses, row pitches (lda, ldb) and group stride (batch_b) are
+ * multiples of 16 bytes, else XF_ERR_MISALIGNED_OPERAND.  The row passes above write rows at any pitch: give an
+ * e4m3 output that feeds a product a pitch of N rounded up to 16.  D may start anywhere.
+ *
  * group_offsets are num_groups + 1 device int32, read by the kernel at each launch: the routing may change
  * between launches of one plan (and of one captured graph) as long as the rows fit M.  They must not
  * decrease; a group may be empty; rows outside [offsets[0], offsets[num_groups]) are neither read for a
@@ -428,8 +432,8 @@ typedef struct xf_grouped_gemm_desc {
   int32_t M, N, K;               /* M: rows of A and D, all groups together; 0 is an empty problem */
   int32_t num_groups;            /* 1..1024 */
   const int32_t* group_offsets;  /* device [num_groups + 1]; NULL with one group: all M rows */
-  const void* A; int64_t lda;                    /* [M][K], K contiguous */
-  const void* B; int64_t ldb; int64_t batch_b;   /* batch_b 0: all groups share one weight */
+  const void* A; int64_t lda;                    /* [M][K], K contiguous; 16-byte aligned rows */
+  const void* B; int64_t ldb; int64_t batch_b;   /* 16-byte aligned rows; batch_b 0: all groups share one weight */
   int32_t b_layout;              /* xf_b_layout */
   int32_t pair;                  /* XF_PAIR_NONE; XF_PAIR_SWIGLU / XF_PAIR_GEGLU: D is [M][N/2], one value
                                     act(v[2j]) * v[2j+1] per pair of columns */

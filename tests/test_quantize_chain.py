@@ -91,3 +91,36 @@ def test_norm_residual_stream_into_a_product(capi, cuda, M, H, K, by_tma):
         slack = (K + 1) * 2 * U * (magnitudes + hs.double().abs())
         assert bool(((Ds.double() - want).abs() <= slack + 2.0 ** -8 * (want.abs() + slack)).all())
     assert plan.device_status() == 0
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 1003, 256), (130, 1003, 264), (33, 129, 72)])
+def test_a_row_pass_of_odd_width_feeds_a_product(capi, cuda, M, K, N):
+    """Rows on 16-byte boundaries (a pitch that is a multiple of 16 codes), as the products' operands need them; with the
+    width as the pitch the pass still writes them and the product refuses them.  128 truncations of 2 u within a block,
+    one rounding per block, four for the factors; the last block is short."""
+    gen = torch.Generator(device="cuda").manual_seed(K + N)
+    e4m3, blocks = torch.float8_e4m3fn, -(-K // 128)
+    x = torch.randn(M, 2 * K, device=cuda, generator=gen).to(torch.bfloat16)
+    q = torch.empty(M, -(-K // 16) * 16, device=cuda, dtype=torch.int8).view(e4m3)[:, :K]
+    scale = torch.empty(blocks, M, device=cuda).t()
+    B = torch.randn(K, -(-N // 16) * 16, device=cuda, generator=gen).mul_(90).to(e4m3)[:, :N]
+    sb = torch.rand(blocks, -(-N // 128), device=cuda, generator=gen) / 64
+    D = torch.empty(M, N, device=cuda)
+    plan = capi.GroupedGemmPlan(q, B, D, scale_a=scale, scale_b=sb)
+
+    def wide(t, dim, n):
+        return t.double().repeat_interleave(128, dim).narrow(dim, 0, n)
+
+    for producer in (lambda: capi.rms_norm_quantize(q, scale, x[:, :K]), lambda: capi.act_mul_quantize(q, scale, x)):
+        producer()
+        plan.run()
+        a, b = q.double() * wide(scale, 1, K), B.double() * wide(wide(sb, 0, K), 1, N)
+        slack = (min(K, 128) * 2 + blocks + 4 + 148) * U * (a.abs() @ b.abs())
+        assert bool(((D.double() - a @ b).abs() <= slack).all())
+    tight = torch.empty(M, K, device=cuda, dtype=torch.int8).view(e4m3)
+    capi.rms_norm_quantize(tight, scale, x[:, :K])
+    capi.rms_norm_quantize(q, scale, x[:, :K])
+    assert torch.equal(tight.double(), q.double())
+    if M > 1:
+        with pytest.raises(capi.XfError, match="16 bytes"):
+            capi.GroupedGemmPlan(tight, B, D, scale_a=scale, scale_b=sb)

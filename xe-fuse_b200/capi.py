@@ -295,7 +295,12 @@ class GroupedGemmPlan:
     A [M, K] and B in bfloat16, or in float8_e4m3fn with scale_a [M, ceil(K/128)] and scale_b; D [M, N]
     ([M, N/2] with a pair op) in bfloat16 or float32.  B is [K, N], or [N, K] with b_nk; scale_b has one value
     for each 128 x 128 block in B's order of dimensions.  With offsets (int32 [G + 1] on the GPU, read at each
-    run) B and scale_b have a leading dimension of G groups, or none: one weight shared by all."""
+    run) B and scale_b have a leading dimension of G groups, or none: one weight shared by all.
+
+    A and B start on 16-byte boundaries, and so do their rows: row pitches are multiples of 16 e4m3 or 8 bf16 elements
+    (a width of 5003: torch.empty(M, 5008)[:, :5003]).  The workspace is cleared on the current stream: a first run on
+    another one has to wait for that (stream.wait_stream(...)), as for the operands.  Runs of one plan must not overlap
+    one another, and a plan lives until its last run has ended: its workspace goes back to the allocator with it."""
 
     def __init__(self, A, B, D, *, offsets=None, scale_a=None, scale_b=None, b_nk=False, pair="none", flags=0):
         import torch

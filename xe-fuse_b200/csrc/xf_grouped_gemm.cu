@@ -276,7 +276,7 @@ xf_status xf_grouped_gemm_plan_create(const xf_grouped_gemm_desc* d, void* works
   }
   memset(plan, 0, sizeof(*plan));
   Params& p = plan->params;
-  const int es = v->kind == KIND_BF16 ? 2 : 1, kblk = 128 / es;
+  const int es = v->kind == KIND_BF16 ? 2 : 1, ds = d->dtype_d == XF_DT_F32 ? 4 : 2, kblk = 128 / es;
   p.M = d->M; p.N = d->N; p.K = d->K; p.G = d->num_groups;
   p.tiles_n = (d->N + v->bn - 1) / v->bn;
   p.num_kb = (d->K + kblk - 1) / kblk;
@@ -293,9 +293,8 @@ xf_status xf_grouped_gemm_plan_create(const xf_grouped_gemm_desc* d, void* works
   p.sa = d->scale_a; p.sa_row = d->scale_a_row_stride; p.sa_blk = d->scale_a_blk_stride;
   p.sb = d->scale_b; p.sb_k = d->scale_b_k_stride; p.sb_n = d->scale_b_n_stride; p.sb_group = d->scale_b_group_stride;
   p.D = d->D; p.ldd = d->ldd;
-  p.d_f32 = d->dtype_d == XF_DT_F32;
   p.pair = d->pair;
-  p.vec_d = grouped::aligned(d->D, 16) && (d->ldd * (p.d_f32 ? 4 : 2)) % 16 == 0;
+  p.vec_d = grouped::aligned(d->D, 16) && (d->ldd * ds) % 16 == 0;
   p.wait_budget = (d->flags & XF_FLAG_SHORT_WAITS) ? 2000000LL : 4000000000LL;
   plan->variant = v;
   plan->fn = g.fn;
@@ -306,12 +305,12 @@ xf_status xf_grouped_gemm_plan_create(const xf_grouped_gemm_desc* d, void* works
     const uint64_t pa = static_cast<uint64_t>(d->lda) * es, pb = static_cast<uint64_t>(d->ldb) * es;
     const int b0 = p.b_nk ? d->K : d->N, b1 = p.b_nk ? d->N : d->K;
     const uint64_t sb = d->batch_b ? static_cast<uint64_t>(d->batch_b) * es : pb * b1;
-    const uint64_t pd = static_cast<uint64_t>(d->ldd) * (p.d_f32 ? 4 : 2);
+    const uint64_t pd = static_cast<uint64_t>(d->ldd) * ds;
     const uint64_t ng = d->batch_b ? d->num_groups : 1;
     if (!encode_3d(&p.tm_a, dt, d->A, d->K, d->M, 1, pa, pa * d->M, kblk, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_3d(&p.tm_a32, dt, d->A, d->K, d->M, 1, pa, pa * d->M, kblk, 32, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        (p.vec_d && !encode_3d(&p.tm_d, p.d_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d->D,
-                               p.pair == XF_PAIR_NONE ? d->N : d->N / 2, d->M, 1, pd, pd * d->M, p.d_f32 ? 16 : 32, 32,
+        (p.vec_d && !encode_3d(&p.tm_d, ds == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d->D,
+                               p.pair == XF_PAIR_NONE ? d->N : d->N / 2, d->M, 1, pd, pd * d->M, 64 / ds, 32,
                                CU_TENSOR_MAP_SWIZZLE_64B)) ||
         !encode_3d(&p.tm_b, dt, d->B, b0, b1, ng, pb, sb, 128 / es, p.b_nk ? 128 : kblk, CU_TENSOR_MAP_SWIZZLE_128B)) {
       free(plan);

@@ -51,7 +51,7 @@ struct alignas(64) Params {
   long long sa_row, sa_blk, sb_k, sb_n, sb_group;
   void* D;
   long long ldd;
-  int d_f32, pair;
+  int pair;
   int vec_d;             // rows of D start on 16-byte boundaries: TMA may write them
   int* status;
   long long wait_budget;

@@ -118,21 +118,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// The same question without waiting for the answer to change: try_wait may suspend the thread for a while.
-__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
 // Bounded wait.  `budget_cycles` is a clock64() budget (a few seconds); the clock is only read
 // every 256 failed polls so the common path costs nothing.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, long long budget_cycles) {

@@ -429,7 +429,8 @@ typedef enum xf_b_layout {
 typedef struct xf_grouped_gemm_desc {
   int32_t dtype_ab;              /* XF_DT_BF16 or XF_DT_E4M3 */
   int32_t dtype_d;               /* XF_DT_BF16 or XF_DT_F32 */
-  int32_t M, N, K;               /* M: rows of A and D, all groups together; 0 is an empty problem */
+  int32_t M, N, K;               /* M: rows of A and D, all groups together; 0 is an empty problem; each at most
+                                    2^31 - 256 */
   int32_t num_groups;            /* 1..1024 */
   const int32_t* group_offsets;  /* device [num_groups + 1]; NULL with one group: all M rows */
   const void* A; int64_t lda;                    /* [M][K], K contiguous; 16-byte aligned rows */

@@ -563,6 +563,24 @@ def test_flags_that_leave_no_tile_are_refused_at_once(capi, bf16, flags, status)
     assert capi.lib().xf_grouped_gemm_can_implement(C.byref(desc(capi, flags=word, **more))) == status
 
 
+@pytest.mark.parametrize("big", [dict(M=2 ** 31 - 255), dict(N=2 ** 31 - 255, ldb=2 ** 31, ldd=2 ** 31),
+                                 dict(K=2 ** 31 - 255, lda=2 ** 31)])
+def test_extents_next_to_32_bits(capi, big):
+    """An extent that leaves 32 bits when it is rounded up to a tile is refused, the largest one that does not is taken."""
+    name = next(iter(big))
+    assert capi.lib().xf_grouped_gemm_can_implement(C.byref(desc(capi, **big))) == 5
+    assert capi.lib().xf_grouped_gemm_can_implement(C.byref(desc(capi, **{**big, name: 2 ** 31 - 256}))) == 0
+
+
+def test_wrapper_refuses_extents_beyond_32_bits(capi, monkeypatch):
+    """They would wrap around in the descriptor."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    A, B, D = torch.zeros(8, 256, dtype=torch.bfloat16), torch.zeros(256, 128, dtype=torch.bfloat16), torch.zeros(8, 128)
+    M = 2 ** 32 + 8
+    with pytest.raises(capi.XfError, match="32-bit"):
+        capi.GroupedGemmPlan(A[:1].expand(M, -1), B, D[:1].expand(M, -1))
+
+
 def test_null_arguments(capi):
     L = capi.lib()
     assert L.xf_grouped_gemm_can_implement(None) == 4

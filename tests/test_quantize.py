@@ -384,3 +384,13 @@ def test_wrapper_refuses_other_dimensions_in_its_own_manner(capi, monkeypatch):
     ):
         with pytest.raises(capi.XfError):
             bad()
+
+
+def test_wrapper_refuses_rows_beyond_32_bits(capi, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    M = 2 ** 31
+    x, s, q = torch.zeros(1, 32, dtype=torch.bfloat16), torch.zeros(1, 1), torch.zeros(1, 32, dtype=E4M3)
+    with pytest.raises(capi.XfError, match="rows"):
+        capi.rms_norm_quantize(q.expand(M, -1), s.expand(M, -1), x.expand(M, -1))
+    with pytest.raises(capi.XfError, match="rows"):
+        capi.act_mul_quantize(q[:, :16].expand(M, -1), s.expand(M, -1), x.expand(M, -1))

@@ -321,6 +321,8 @@ class GroupedGemmPlan:
         M, K = A.shape
         N = B.shape[-2] if b_nk else B.shape[-1]
         G = offsets.shape[0] - 1 if offsets is not None else 1
+        if max(M, N, K) >> 31:
+            raise XfError(5, f"extents are 32-bit: M={M} N={N} K={K}")
         lead = () if B.dim() == 2 else (G,)
         lda = _rows(A, "A", (M, K), A.dtype, device)
         ldd = _rows(D, "D", (M, N if pair == "none" else N // 2), D.dtype, device)
@@ -537,6 +539,8 @@ def _codes(out, scale, shape, device):
     if len(shape) != 2:
         raise XfError(3, f"expected a matrix, got shape {tuple(shape)}")
     dtype, (M, N), st = out.dtype, shape, scale.stride()
+    if M >> 31:
+        raise XfError(5, f"at most 2^31 - 1 rows, got {M}")
     if dtype == torch.float8_e4m3fn:
         code, want = DT_E4M3, (M, -(-N // 128))
     elif dtype == torch.int8:

@@ -43,6 +43,10 @@ static xf_status validate(const xf_grouped_gemm_desc* d) {
     set_error("problem extents must be positive (M=%d N=%d K=%d groups=%d)", d->M, d->N, d->K, d->num_groups);
     return XF_ERR_INVALID_PROBLEM;
   }
+  if (d->M > kMaxExtent || d->N > kMaxExtent || d->K > kMaxExtent) {
+    set_error("extents of at most %d (M=%d N=%d K=%d)", kMaxExtent, d->M, d->N, d->K);
+    return XF_ERR_NOT_SUPPORTED;
+  }
   if (d->num_groups > kMaxGroups) {
     set_error("at most %d groups (got %d)", kMaxGroups, d->num_groups);
     return XF_ERR_NOT_SUPPORTED;
@@ -152,7 +156,8 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
   //         128 x 128, one CTA   600  2000  3000   900
   // Large tiles read fewer operand bytes per multiplication; tiles of 128 rows waste less on groups of few
   // rows, and small ones spread better.  Rows of a group are taken to fill half of its last tile.  e4m3, pair /
-  // 128 x 256 / 128 x 128: 4096 x 28672 x 4096 402 / 446 / 530 us, 777 x 5001 x 2000 34 / 20 / 24 us,
+  // 128 x 256 / 128 x 128, in bursts of 30 launches (back to back under the power cap: 464 us and 243 us for the tiles
+  // that the rule takes in the first and third case): 4096 x 28672 x 4096 402 / 446 / 530 us, 777 x 5001 x 2000 34 / 20 / 24 us,
   // 64 experts 16384 x 4096 x 2048 262 / 215 / 236 us, 100 x 8192 x 8192 - / 23 / 16.5 us.
   const Variant* v = nullptr;
   int count = 0;

@@ -30,6 +30,7 @@ namespace xf {
 namespace grouped {
 
 static const int kMaxGroups = 1024;
+static const int kMaxExtent = 0x7FFFFF00;   // an extent rounded up to a tile's edge stays within 32 bits
 static const int kTileList = 128;   // tiles of a unit that are looked up once, when the kernel starts
 enum : int { KIND_BF16 = 0, KIND_E4M3 = 2 };   // the KIND of ptx::umma
 // What a kernel instance writes.  One instance for each: the code of another form, never run, takes registers

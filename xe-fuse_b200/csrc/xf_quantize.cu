@@ -12,9 +12,12 @@
 // The floor of 2^-100 gives a block of zeros zero codes and keeps L / a finite.  Maxima are taken over the bit
 // patterns without the sign, so a NaN is the largest of all and reaches the scale of its block.
 //
-// Bound.  Each byte moves once: 7 bytes per element with a residual (x, r in; h, code out), 5 per output
-// element of the gated form.  Long inputs run at 5.5 TB/s (4096 x 8192 42.5 us, 4096 x 14336 54 us), between HBM's
-// 6.5 and the issue slots' limit (about 21 instructions per column).
+// Bound.  Each byte moves once, 7 bytes per element with a residual (x, r in; h, code out), 5 per output element of
+// the gated form, except in int8 rows that shared memory does not hold (see kRowBytes), which are read twice.  e4m3
+// (4096 x 8192 with residual 42.4 us, 4096 x 14336 SiLU 53.8 us) runs at 5.5 TB/s, 0.84 of the copy rate, with issue
+// slots 54 % and 64 % busy and warps waiting for loads most: too few of them in flight.  GeLU (77.7 us) is bound by issue
+// slots, 92 % busy at 45 instructions per column.  int8 rows run well below either bound (4096 x 8192 68 us,
+// 4096 x 14336 SiLU 124 us): 84 registers in the norm, 2 blocks per SM, and a second pass over each row.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -334,8 +337,8 @@ __device__ __forceinline__ void gated(const Chunk& g, const Chunk& u, float (&y)
 
 // e4m3: kLanes lanes per block of 128 columns; nothing is shared beyond them.  A thread block works in one
 // row, `segs` of them on each: the row comes from one uniform division.  Sixteen columns per thread halve
-// what a block's maximum, division and addresses cost per column: the kernel is issue-bound (28 instructions
-// per column with eight, 59 -> 54 us at 4096 x 14336, 5.5 TB/s).
+// what a block's maximum, division and addresses cost per column: 28 instructions with eight, 21 with sixteen
+// (59 -> 54 us at 4096 x 14336, 5.5 TB/s).
 template <bool GELU>
 __global__ void __launch_bounds__(256) act_mul_e4m3_kernel(const Params p, unsigned segs) {
   ptx::griddep_launch_dependents();
@@ -485,14 +488,17 @@ static xf_status launch(const char* what, void (*fn)(Args...), unsigned grid, un
 }
 
 // Threads for a row: one chunk each where there are few rows, kAhead where other rows keep the SM busy
-// (4096 x 8192 with residual: 42.7 us, 5.5 TB/s; four chunks each 52 us).
+// (4096 x 8192 with residual: 42.4 us, 5.5 TB/s; four chunks each 52 us).
 static unsigned row_threads(int M, int N) {
   const int chunks = (N + kChunk - 1) / kChunk, each = M >= 512 ? kAhead : 1;
   const int t = ((chunks + each - 1) / each + 31) / 32 * 32;
   return t > 512 ? 512 : t;
 }
 
-static const int kRowBytes = 47 * 1024;   // rows up to this size wait in shared memory (48 KB need no opt-in)
+// int8 rows up to this size wait in shared memory (48 KB need no opt-in): 24064 columns of the norm, 12032 of the gate,
+// whose products wait in fp32.  Longer ones are read and, in the gate, activated twice: 4096 x 11008 66 us,
+// 4096 x 14336 124 us.
+static const int kRowBytes = 47 * 1024;
 
 }  // namespace quantize
 }  // namespace xf

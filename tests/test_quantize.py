@@ -394,3 +394,11 @@ def test_wrapper_refuses_rows_beyond_32_bits(capi, monkeypatch):
         capi.rms_norm_quantize(q.expand(M, -1), s.expand(M, -1), x.expand(M, -1))
     with pytest.raises(capi.XfError, match="rows"):
         capi.act_mul_quantize(q[:, :16].expand(M, -1), s.expand(M, -1), x.expand(M, -1))
+
+
+def test_a_residual_out_without_a_residual_is_refused(capi, monkeypatch):
+    """It was left as it is without a word."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    x, s, q = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(4, 2), torch.zeros(4, 256, dtype=E4M3)
+    with pytest.raises(capi.XfError, match="residual"):
+        capi.rms_norm_quantize(q, s, x, residual_out=torch.zeros_like(x))

@@ -570,6 +570,8 @@ def rms_norm_quantize(out, scale, inp, weight=None, residual=None, residual_out=
             residual_out = residual
         rp, rl = residual.data_ptr(), _rows(residual, "residual", shape, bf16, device)
         hp, hl = residual_out.data_ptr(), _rows(residual_out, "residual_out", shape, bf16, device)
+    elif residual_out is not None:
+        raise XfError(4, "residual_out is written only where there is a residual")
     if weight is not None:
         wp = weight.data_ptr()
         if (weight.dtype, weight.shape, weight.get_device()) != (bf16, (N,), device) or not weight.is_contiguous():

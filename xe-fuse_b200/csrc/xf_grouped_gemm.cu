@@ -156,9 +156,9 @@ static xf_status plan_geometry(const xf_grouped_gemm_desc* d, Geometry* g) {
   //         128 x 128, one CTA   600  2000  3000   900
   // Large tiles read fewer operand bytes per multiplication; tiles of 128 rows waste less on groups of few
   // rows, and small ones spread better.  Rows of a group are taken to fill half of its last tile.  e4m3, pair /
-  // 128 x 256 / 128 x 128, in bursts of 30 launches (back to back under the power cap: 464 us and 243 us for the tiles
-  // that the rule takes in the first and third case): 4096 x 28672 x 4096 402 / 446 / 530 us, 777 x 5001 x 2000 34 / 20 / 24 us,
-  // 64 experts 16384 x 4096 x 2048 262 / 215 / 236 us, 100 x 8192 x 8192 - / 23 / 16.5 us.
+  // 128 x 256 / 128 x 128, in bursts of 30 launches: 4096 x 28672 x 4096 407 / 429 / 539 us, 777 x 5001 x 2000
+  // 35 / 21 / 25 us, 64 experts 16384 x 4096 x 2048 268 / 216 / 242 us, 100 x 8192 x 8192 - / 23 / 16.5 us.  (Back to
+  // back, under the power cap, the first takes 464 us and the third 243 us with the tiles chosen here.)
   const Variant* v = nullptr;
   int count = 0;
   const Variant* all = tiles_of(d->dtype_ab, &count);

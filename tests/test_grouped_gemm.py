@@ -437,6 +437,34 @@ def test_plans_on_two_streams_meet_new_data(capi, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [E4M3, torch.bfloat16])
+def test_shared_tiles_beside_other_work(capi, cuda, dtype):
+    """While large products of another stream hold SMs, a launch's CTAs start one after another: those that collect
+    partial sums only wait for CTAs of lower index, which have started before them."""
+    sets = [make(300, 700, 8000, dtype=dtype, seed=s) for s in (1, 2, 3)]
+    a = torch.randn(8192, 8192, device=cuda).to(torch.bfloat16)
+    op = make(300, 700, 8000, dtype=dtype, seed=4)
+    D = torch.empty(300, 700, device=cuda)
+    side = torch.cuda.Stream()
+    for flags in [f for f in tiles(capi, dtype) if not f & capi.FLAG_NO_SPLIT]:
+        plan = capi.GroupedGemmPlan(op["A"], op["B"], D, scale_a=op.get("scale_a"), scale_b=op.get("scale_b"), flags=flags)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(4):
+                b = a @ a
+        got = []
+        for i in range(12):
+            renew(op, sets[i % 3])
+            D.fill_(-7.0)
+            plan.run()
+            got.append(D.clone())
+        torch.cuda.synchronize()
+        assert plan.device_status() == 0
+        for i, D_i in enumerate(got):
+            check(sets[i % 3], D_i, "none", D_i)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("experts", [False, True])
 def test_feed_forward_in_8_bits(capi, cuda, experts):
     """norm + quantise -> gate/up product -> activation + quantise -> down product, captured in one graph."""

@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(384, 1) grouped_gemm_kernel(const __grid_const
         begun.issued = issued;
         begun.filled = filled;
       }
-      }
+    }
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ promotion and epilogue
     if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
